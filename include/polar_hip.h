@@ -6,7 +6,7 @@
  * Everything here is plain C: opaque handles, raw device pointers, 64-bit
  * element counts.  All tensors are dense, row-major fp32, exactly as the
  * reference's runtimes see them (src/backend/generic/runtime/sycl/kernels/
- * common.hpp:35-38).  Kernel entry points enqueue work on the device's stream
+ * common.hpp:35-38); the operators at the end say what else they take.  Kernel entry points enqueue work on the device's stream
  * and return without waiting; ordering is stream order.
  *
  * Return value of every function that returns int: 0 on success, otherwise a
@@ -321,6 +321,112 @@ int polar_hip_fmatmul_fadd_fsigmoid(polar_hip_device* dev, int transA,
 int polar_hip_fsigmoid_flogloss(polar_hip_device* dev, const float* in,
                                 const float* groundTruth, float* out,
                                 uint64_t n);
+
+/* ---- Operators of a language model's training step and sampling loop ------------
+ * No counterpart in the reference, whose graphs end at fsoftmax over a whole
+ * tensor, flogloss and the update W <- W + lr * grad.  They take their tensors
+ * in fp32, fp16 or bf16 and compute in fp32; a matrix is given by its first
+ * element, the distance of two rows' first elements (its stride, in elements,
+ * at least cols) and rows x cols, and its elements behind cols in a row are
+ * neither read nor written.  Pointers need the alignment of one element.  Rows
+ * may be none; then nothing is done. */
+typedef enum polar_hip_type { POLAR_HIP_F32 = 0, POLAR_HIP_F16 = 1, POLAR_HIP_BF16 = 2 } polar_hip_type;
+/* Tokens: whole numbers, also as fp32 (the framework's tensors hold nothing else) */
+typedef enum polar_hip_index_type {
+  POLAR_HIP_INDEX_I32 = 0,
+  POLAR_HIP_INDEX_I64 = 1,
+  POLAR_HIP_INDEX_F32 = 2
+} polar_hip_index_type;
+
+/* flayernorm: y = (x - mean) * rstd * weight + bias for each row of x, with
+ * rstd = 1 / sqrt(variance + eps) and the variance over cols elements (1 to
+ * 2^24).  weight and bias (cols elements of paramType: fp32 or x's type) may
+ * be null: ones and zeros.  mean and rstd (rows elements) are what the
+ * gradient wants of this pass; either may be null.  y may be x (equal
+ * strides). */
+int polar_hip_flayernorm(polar_hip_device* dev, int type, const void* x,
+                         uint64_t xStride, int paramType, const void* weight,
+                         const void* bias, float eps, void* y, uint64_t yStride,
+                         float* mean, float* rstd, uint64_t rows, uint64_t cols);
+/* flayernorm_grad: dx, dweight and dbias (of paramType, summed in fp32 over the
+ * rows in an order that the sizes fix, rounded once) from dy; any of the three
+ * may be null.  mean and rstd come from flayernorm; both null: they are computed
+ * again from x with eps (x is read anyway).  dx may be dy or x (equal strides). */
+int polar_hip_flayernorm_grad(polar_hip_device* dev, int type, const void* dy,
+                              uint64_t dyStride, const void* x, uint64_t xStride,
+                              int paramType, const void* weight,
+                              const float* mean, const float* rstd, float eps,
+                              void* dx, uint64_t dxStride, void* dweight,
+                              void* dbias, uint64_t rows, uint64_t cols);
+
+#define POLAR_HIP_LOGPROB_MAX_TOP 32
+/* flogprob: for each row of logits (1 to 2^24 of them), of the distribution
+ * softmax(scale * logits), scale > 0:
+ *   logprob[row]  log probability of tokens[row]; 0 where the token is negative
+ *                 (a place that does not count), NaN where it is >= cols
+ *   stats[row]    two values that flogprob_grad wants: the largest logit, and the
+ *                 log of the sum of exp(scale * (logit - largest)); the log of
+ *                 sum of exp(scale * logit) is scale * stats[0] + stats[1]
+ *   entropy[row]  -sum p log p
+ *   topIndex, topLogprob [row][top]  the `top` (0 to 32, at most cols) likeliest
+ *                 tokens in order, of equal logits the lowest first, and their
+ *                 log probabilities
+ * Each output may be null (topIndex and topLogprob where top is 0).  -infinity
+ * is a logit that is ruled out.  A row of nothing else: log probabilities
+ * -infinity, entropy 0, stats both -infinity.  A row with a NaN or +infinity:
+ * log probabilities, entropy and stats[1] NaN, topIndex -1. */
+int polar_hip_flogprob(polar_hip_device* dev, int type, const void* logits,
+                       uint64_t stride, int tokenType, const void* tokens,
+                       float scale, float* logprob, float* stats, float* entropy,
+                       uint32_t top, int32_t* topIndex, float* topLogprob,
+                       uint64_t rows, uint64_t cols);
+/* flogprob_grad: dlogits from the gradients with regard to logprob and entropy
+ * (either may be null: zeros).  stats, and entropy where dentropy is given, come
+ * from flogprob with the same logits and scale.  A row whose token is negative
+ * has no share of dlogprob, a row of -infinity alone gets zeros, a row whose token
+ * is >= cols NaN.  dlogits may be logits (equal strides). */
+int polar_hip_flogprob_grad(polar_hip_device* dev, int type, const void* logits,
+                            uint64_t stride, int tokenType, const void* tokens,
+                            float scale, const float* stats,
+                            const float* dlogprob, const float* entropy,
+                            const float* dentropy, void* dlogits,
+                            uint64_t dlogitsStride, uint64_t rows, uint64_t cols);
+
+/* Elements that share a scale where AdamW's states are held in 8 bits */
+#define POLAR_HIP_ADAMW_BLOCK 256
+typedef struct polar_hip_adamw_tensor {
+  void* param;        /* count elements of param_type                             */
+  const void* grad;   /* count elements of grad_type                              */
+  void* m;            /* first moment: fp32, or 8-bit floats (sign, 4 exponent and */
+                      /* 3 mantissa bits, largest 448) that m_scale multiplies     */
+  void* v;            /* second moment: fp32, or its square root as such floats    */
+  float* master;      /* param_type fp32: not used.  Otherwise the parameters in   */
+                      /* fp32, of which param gets a rounded copy                  */
+  float* m_scale;     /* 8-bit states: one per 256 elements; else not used         */
+  float* v_scale;
+  uint64_t count;     /* may be 0: the tensor is passed over                      */
+  uint64_t first;     /* number of the tensor's first element in the sequence of   */
+                      /* random numbers: the elements of the tensors before it     */
+  double weight_decay;
+} polar_hip_adamw_tensor;
+typedef struct polar_hip_adamw_config {
+  int param_type, grad_type; /* polar_hip_type */
+  int state_bits;            /* 32 or 8 */
+  uint32_t seed;             /* 8-bit states: of the stochastic rounding; another for each step */
+  int64_t step;              /* 1 for the first */
+  double lr, beta1, beta2, eps;
+  double grad_scale;         /* gradients are multiplied by it first */
+} polar_hip_adamw_config;
+/* fadamw: one step over `count` tensors, each updated in place:
+ *   g = grad_scale * grad;  m = beta1 m + (1 - beta1) g;  v = beta2 v + (1 - beta2) g^2
+ *   param = param - lr weight_decay param
+ *           - lr / (1 - beta1^step) m / (sqrt(v) / sqrt(1 - beta2^step) + eps)
+ * The list is read before the call returns.  All of it is checked before
+ * anything is launched.  Tensors must not overlap.  8-bit states are rounded
+ * stochastically, up where the upper (v) or lower (m) 16 bits of a hash of seed
+ * and element number say so; a block whose scale is below 2^-100 holds zeros. */
+int polar_hip_fadamw(polar_hip_device* dev, const polar_hip_adamw_config* config,
+                     const polar_hip_adamw_tensor* tensors, uint64_t count);
 
 #ifdef __cplusplus
 }

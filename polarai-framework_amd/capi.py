@@ -46,8 +46,45 @@ class PoolStats(C.Structure):
     ]
 
 
+class AdamWTensor(C.Structure):
+    _fields_ = [
+        ("param", C.c_void_p),
+        ("grad", C.c_void_p),
+        ("m", C.c_void_p),
+        ("v", C.c_void_p),
+        ("master", C.c_void_p),
+        ("m_scale", C.c_void_p),
+        ("v_scale", C.c_void_p),
+        ("count", C.c_uint64),
+        ("first", C.c_uint64),
+        ("weight_decay", C.c_double),
+    ]
+
+
+class AdamWConfig(C.Structure):
+    _fields_ = [
+        ("param_type", C.c_int),
+        ("grad_type", C.c_int),
+        ("state_bits", C.c_int),
+        ("seed", C.c_uint32),
+        ("step", C.c_int64),
+        ("lr", C.c_double),
+        ("beta1", C.c_double),
+        ("beta2", C.c_double),
+        ("eps", C.c_double),
+        ("grad_scale", C.c_double),
+    ]
+
+
+TYPES = {"f32": 0, "f16": 1, "bf16": 2}         # polar_hip_type
+INDEX_TYPES = {"i32": 0, "i64": 1, "f32": 2}    # polar_hip_index_type
+STATE_BITS = {"f32": 32, "8bit": 8}
+LOGPROB_MAX_TOP = 32
+ADAMW_BLOCK = 256
+
 _vp = C.c_void_p
 _u64 = C.c_uint64
+_u32 = C.c_uint32
 _f = C.c_float
 _i = C.c_int
 
@@ -104,6 +141,12 @@ SIGNATURES = {
     "polar_hip_fmatmul_fsigmoid": (_i, [_vp, _i, _i, _vp, _vp, _vp, _u64, _u64, _u64]),
     "polar_hip_fmatmul_fadd_fsigmoid": (_i, [_vp, _i, _i, _vp, _vp, _f, _vp, _f, _vp, _u64, _u64, _u64]),
     "polar_hip_fsigmoid_flogloss": (_i, [_vp, _vp, _vp, _vp, _u64]),
+    "polar_hip_flayernorm": (_i, [_vp, _i, _vp, _u64, _i, _vp, _vp, _f, _vp, _u64, _vp, _vp, _u64, _u64]),
+    "polar_hip_flayernorm_grad": (_i, [_vp, _i, _vp, _u64, _vp, _u64, _i, _vp, _vp, _vp, _f, _vp, _u64, _vp, _vp,
+                                       _u64, _u64]),
+    "polar_hip_flogprob": (_i, [_vp, _i, _vp, _u64, _i, _vp, _f, _vp, _vp, _vp, _u32, _vp, _vp, _u64, _u64]),
+    "polar_hip_flogprob_grad": (_i, [_vp, _i, _vp, _u64, _i, _vp, _f, _vp, _vp, _vp, _vp, _vp, _u64, _u64, _u64]),
+    "polar_hip_fadamw": (_i, [_vp, C.POINTER(AdamWConfig), C.POINTER(AdamWTensor), _u64]),
 }
 
 _lib = None
@@ -131,6 +174,33 @@ def load_library(path=LIB_DEVICE):
 def _check(lib, status):
     if status != 0:
         raise PolarHipError(status, lib.polar_hip_last_error().decode())
+
+
+def _ptr(x):
+    """Device address of a Buffer, of a tensor of another library on the same GPU (anything with data_ptr()), or of
+    a plain address; None stays None.  The device's stream is its own: work of another library on such a tensor is
+    waited for before the call, and the call before that library uses the tensor again."""
+    if x is None or isinstance(x, int):
+        return x
+    at = getattr(x, "ptr", None)
+    return x.data_ptr() if at is None else at
+
+
+def adamw_tensors(tensors):
+    """The list of tensors that Device.fadamw takes, from dicts with the fields of polar_hip_adamw_tensor (those left
+    out or None are null; weight_decay is 0).  A training program makes it once."""
+    table = (AdamWTensor * len(tensors))()
+    for entry, t in zip(table, tensors):
+        for name, value in t.items():
+            if name in ("count", "first"):
+                setattr(entry, name, int(value))
+            elif name == "weight_decay":
+                entry.weight_decay = value
+            elif name in ("param", "grad", "m", "v", "master", "m_scale", "v_scale"):
+                setattr(entry, name, _ptr(value))
+            else:
+                raise KeyError(f"no field {name} in a tensor of fadamw")
+    return table
 
 
 def fpool_plan(height, width, window, stride, input_aligned=True):
@@ -370,3 +440,40 @@ class Device:
     def fmatmul(self, trans_a, trans_b, a, b, c, m, n, k):
         _check(self.lib, self.lib.polar_hip_fmatmul(
             self.handle, int(bool(trans_a)), int(bool(trans_b)), a.ptr, b.ptr, c.ptr, m, n, k))
+
+    # -- operators of a language model's training step and sampling loop (asynchronous) --
+    # tensors are Buffers, tensors of another library, or device addresses (_ptr)
+    def flayernorm(self, x, weight, bias, out, rows, cols, eps=1e-5, mean=None, rstd=None, dtype="f32",
+                   param_dtype="f32", x_stride=None, out_stride=None):
+        _check(self.lib, self.lib.polar_hip_flayernorm(
+            self.handle, TYPES[dtype], _ptr(x), cols if x_stride is None else x_stride, TYPES[param_dtype],
+            _ptr(weight), _ptr(bias), eps, _ptr(out), cols if out_stride is None else out_stride, _ptr(mean),
+            _ptr(rstd), rows, cols))
+
+    def flayernorm_grad(self, grad, x, weight, dx, dweight, dbias, rows, cols, eps=1e-5, mean=None, rstd=None,
+                        dtype="f32", param_dtype="f32", grad_stride=None, x_stride=None, dx_stride=None):
+        _check(self.lib, self.lib.polar_hip_flayernorm_grad(
+            self.handle, TYPES[dtype], _ptr(grad), cols if grad_stride is None else grad_stride, _ptr(x),
+            cols if x_stride is None else x_stride, TYPES[param_dtype], _ptr(weight), _ptr(mean), _ptr(rstd), eps,
+            _ptr(dx), cols if dx_stride is None else dx_stride, _ptr(dweight), _ptr(dbias), rows, cols))
+
+    def flogprob(self, logits, tokens, logprob, rows, cols, scale=1.0, stats=None, entropy=None, top=0, top_index=None,
+                 top_logprob=None, dtype="f32", token_dtype="i64", stride=None):
+        _check(self.lib, self.lib.polar_hip_flogprob(
+            self.handle, TYPES[dtype], _ptr(logits), cols if stride is None else stride, INDEX_TYPES[token_dtype],
+            _ptr(tokens), scale, _ptr(logprob), _ptr(stats), _ptr(entropy), top, _ptr(top_index), _ptr(top_logprob),
+            rows, cols))
+
+    def flogprob_grad(self, logits, tokens, stats, dlogprob, dlogits, rows, cols, scale=1.0, entropy=None,
+                      dentropy=None, dtype="f32", token_dtype="i64", stride=None, dlogits_stride=None):
+        _check(self.lib, self.lib.polar_hip_flogprob_grad(
+            self.handle, TYPES[dtype], _ptr(logits), cols if stride is None else stride, INDEX_TYPES[token_dtype],
+            _ptr(tokens), scale, _ptr(stats), _ptr(dlogprob), _ptr(entropy), _ptr(dentropy), _ptr(dlogits),
+            cols if dlogits_stride is None else dlogits_stride, rows, cols))
+
+    def fadamw(self, tensors, step, lr, beta1=0.9, beta2=0.999, eps=1e-8, grad_scale=1.0, seed=0, dtype="f32",
+               grad_dtype="f32", state_dtype="f32"):
+        """`tensors`: what adamw_tensors() made."""
+        config = AdamWConfig(TYPES[dtype], TYPES[grad_dtype], STATE_BITS[state_dtype], seed, step, lr, beta1, beta2, eps,
+                             grad_scale)
+        _check(self.lib, self.lib.polar_hip_fadamw(self.handle, C.byref(config), tensors, len(tensors)))

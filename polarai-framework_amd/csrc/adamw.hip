@@ -1,0 +1,302 @@
+// One AdamW step over a list of tensors, with states in 32 or in 8 bits.
+//
+//   g = gradScale * grad,  m = b1 m + (1 - b1) g,  v = b2 v + (1 - b2) g^2
+//   p = p - lr wd p - (lr / (1 - b1^t)) m / (sqrt(v) / sqrt(1 - b2^t) + eps)
+//
+// Everything is read once and written once.  A launch covers up to kTensors
+// tensors, whose table travels in the kernel's arguments: no table in device
+// memory to upload and keep, and a model of a few hundred tensors takes a few
+// launches.  A work-group takes a chunk of kChunk elements of one tensor; a
+// lane takes four consecutive elements at a time.
+//
+// States in 8 bits: 256 consecutive elements of a tensor (one wave's four per
+// lane) share a scale, the largest value in the block / 448.  m is held as an
+// 8-bit float (sign, four exponent bits, three mantissa bits; 448 is its
+// largest), and so is sqrt(v) rather than v: its range of 2^18 spans 2^36 in v.
+// Rounding is stochastic: a value between two neighbours goes up with the
+// probability of its distance to the lower one.  To nearest, v would stand
+// still: a step moves it by (1 - b2) = 0.1 %, far less than half the distance
+// of two neighbours (3 to 6 %); stochastically it follows on average.  The 16
+// random bits come from a hash of the caller's seed and the element's number.
+// The parameter is updated from the unrounded states.
+#include "typed.h"
+
+#include <algorithm>
+#include <cmath>
+
+using namespace polar_hip_detail;
+
+namespace {
+
+constexpr int kBlock = 256;
+constexpr int kRounds = 4;                          // groups of four elements per lane
+constexpr uint32_t kChunk = kBlock * 4 * kRounds;   // elements of a work-group
+constexpr uint64_t kScaleBlock = POLAR_HIP_ADAMW_BLOCK; // elements that share a scale
+static_assert(kScaleBlock == 64 * 4, "one wave's four elements per lane");
+constexpr float kLargest = 448.0f;                  // of the 8-bit floats
+constexpr float kTiny = 0x1p-100f;                  // blocks whose scale is not above this are held as zeros
+
+constexpr int kTensors = 40;
+struct Entry {
+  void *param, *grad, *m, *v;
+  float *master, *mScale, *vScale;
+  uint64_t count, random;
+  float decay; // lr * weight decay
+};
+struct Table {
+  Entry e[kTensors];
+  uint32_t firstGroup[kTensors]; // of each tensor; the largest number behind the last one
+  float gradScale, beta1, rest1, beta2, rest2, stepSize, byCorrection, eps;
+  uint32_t seed;
+};
+static_assert(sizeof(Table) <= 4000, "kernel arguments");
+
+template <int kBytes> struct Words;
+template <> struct Words<16> { typedef uint32_t At __attribute__((ext_vector_type(4), aligned(4))); };
+template <> struct Words<8> { typedef uint32_t At __attribute__((ext_vector_type(2), aligned(2))); };
+
+// four consecutive elements, the first `n` of them real (1 .. 4)
+template <typename T>
+__device__ __forceinline__ void load4(const typename T::Stored* at, int n, float* out) {
+  using S = typename T::Stored;
+  S v[4];
+  if (n == 4) {
+    const auto w = __builtin_nontemporal_load(reinterpret_cast<const typename Words<4 * sizeof(S)>::At*>(at));
+    __builtin_memcpy(v, &w, sizeof(v));
+  } else {
+#pragma unroll
+    for (int i = 0; i < 4; ++i) v[i] = i < n ? at[i] : S(0.0f);
+  }
+#pragma unroll
+  for (int i = 0; i < 4; ++i) out[i] = T::widen(v[i]);
+}
+template <typename T>
+__device__ __forceinline__ void store4(typename T::Stored* at, int n, const float* x) {
+  using S = typename T::Stored;
+  S v[4];
+#pragma unroll
+  for (int i = 0; i < 4; ++i) v[i] = T::narrow(x[i]);
+  if (n == 4) {
+    using At = typename Words<4 * sizeof(S)>::At;
+    At w;
+    __builtin_memcpy(&w, v, sizeof(v));
+    __builtin_nontemporal_store(w, reinterpret_cast<At*>(at));
+  } else {
+#pragma unroll
+    for (int i = 0; i < 4; ++i)
+      if (i < n) at[i] = v[i];
+  }
+}
+
+typedef uint32_t WordAt1 __attribute__((aligned(1)));
+__device__ __forceinline__ uint32_t loadCodes(const uint8_t* at, int n) {
+  if (n == 4) return __builtin_nontemporal_load(reinterpret_cast<const WordAt1*>(at));
+  uint32_t w = 0;
+#pragma unroll
+  for (int i = 0; i < 4; ++i) w |= i < n ? uint32_t(at[i]) << (8 * i) : 0u;
+  return w;
+}
+__device__ __forceinline__ void storeCodes(uint8_t* at, int n, uint32_t w) {
+  if (n == 4) {
+    __builtin_nontemporal_store(w, reinterpret_cast<WordAt1*>(at));
+  } else {
+#pragma unroll
+    for (int i = 0; i < 4; ++i)
+      if (i < n) at[i] = static_cast<uint8_t>(w >> (8 * i));
+  }
+}
+__device__ __forceinline__ void widenCodes(uint32_t w, float* out) {
+  const Float2 low = __builtin_amdgcn_cvt_pk_f32_fp8(w, false), high = __builtin_amdgcn_cvt_pk_f32_fp8(w, true);
+  out[0] = low.x, out[1] = low.y, out[2] = high.x, out[3] = high.y;
+}
+// |t| <= 448 as an 8-bit float, up where 16 random bits exceed what is cut off:
+// among the normal ones by adding them below the mantissa's last kept bit (the
+// carry may reach the exponent, which is the next float), below 2^-6 in steps of
+// 2^-9
+__device__ __forceinline__ uint32_t narrowCode(float t, uint32_t random) {
+  const float size = fabsf(t);
+  const uint32_t normal = ((__builtin_bit_cast(uint32_t, size) + (random << 4)) >> 20) - (120u << 3);
+  const uint32_t small = static_cast<uint32_t>(size * 512.0f + static_cast<float>(random) * (1.0f / 65536.0f));
+  const uint32_t code = size >= 0x1p-6f ? (normal < 0x7eu ? normal : 0x7eu) : small;
+  return code | (t < 0.0f ? 0x80u : 0u);
+}
+
+// 32 random bits of an element: a multiply-xorshift hash of its number and the
+// seed (two rounds with the odd constants of the 32-bit finaliser of MurmurHash3,
+// published by its author Austin Appleby into the public domain)
+__device__ __forceinline__ uint32_t randomBits(uint32_t seed, uint64_t element) {
+  uint32_t h = static_cast<uint32_t>(element) * 0x9e3779b1u + static_cast<uint32_t>(element >> 32) * 0x85ebca77u + seed;
+  h = (h ^ (h >> 16)) * 0x85ebca6bu;
+  h = (h ^ (h >> 13)) * 0xc2b2ae35u;
+  return h ^ (h >> 16);
+}
+
+// P: the parameter's type; one of 16 bits is a copy of the fp32 master.  G: the gradient's.
+template <typename P, typename G, bool kSmall>
+__global__ __launch_bounds__(kBlock) void adamwKernel(Table table) {
+  constexpr bool kCopy = sizeof(typename P::Stored) == 2;
+  // all the first groups sit side by side in scalar registers: no search through memory
+  int which = 0;
+  uint32_t first = 0;
+#pragma unroll
+  for (int i = 1; i < kTensors; ++i) {
+    const bool behind = blockIdx.x >= table.firstGroup[i];
+    which += behind;
+    first = behind ? table.firstGroup[i] : first;
+  }
+  const Entry e = table.e[which];
+  const uint64_t base = uint64_t(blockIdx.x - first) * kChunk + threadIdx.x * 4;
+  float* master = kCopy ? e.master : static_cast<float*>(e.param);
+#pragma unroll
+  for (int round = 0; round < kRounds; ++round) {
+    const uint64_t at = base + uint64_t(round) * kBlock * 4;
+    const int n = at >= e.count ? 0 : e.count - at < 4 ? static_cast<int>(e.count - at) : 4;
+    // a wave whose block of 256 lies behind the tensor's end has nothing to do
+    if (kSmall ? at - threadIdx.x % 64 * 4 >= e.count : n == 0) break;
+    float p[4], g[4], m[4], v[4], r[4];
+    const uint64_t block = at / kScaleBlock;
+    if constexpr (kSmall) {
+      const float ms = e.mScale[block], vs = e.vScale[block];
+      widenCodes(n ? loadCodes(static_cast<const uint8_t*>(e.m) + at, n) : 0u, m);
+      widenCodes(n ? loadCodes(static_cast<const uint8_t*>(e.v) + at, n) : 0u, r);
+#pragma unroll
+      for (int i = 0; i < 4; ++i) {
+        m[i] *= ms;
+        r[i] *= vs;
+        v[i] = r[i] * r[i];
+      }
+    } else {
+      load4<TypeF32>(static_cast<const float*>(e.m) + at, n, m);
+      load4<TypeF32>(static_cast<const float*>(e.v) + at, n, v);
+    }
+    load4<TypeF32>(master + at, n, p);
+    load4<G>(static_cast<const typename G::Stored*>(e.grad) + at, n, g);
+#pragma unroll
+    for (int i = 0; i < 4; ++i) {
+      g[i] *= table.gradScale;
+      m[i] = m[i] * table.beta1 + g[i] * table.rest1;
+      v[i] = v[i] * table.beta2 + (g[i] * g[i]) * table.rest2;
+      r[i] = sqrtf(v[i]);
+      p[i] = (p[i] - p[i] * e.decay) - (m[i] * table.stepSize) / (r[i] * table.byCorrection + table.eps);
+    }
+    if (n) {
+      store4<TypeF32>(master + at, n, p);
+      if constexpr (kCopy) store4<P>(static_cast<typename P::Stored*>(e.param) + at, n, p);
+    }
+    if constexpr (kSmall) {
+      // elements behind the end are zeros: loads give them as such, and they stay
+      float largestM = 0.0f, largestR = 0.0f;
+#pragma unroll
+      for (int i = 0; i < 4; ++i) {
+        largestM = fmaxf(largestM, fabsf(m[i]));
+        largestR = fmaxf(largestR, r[i]);
+      }
+      const float ms = waveMax(largestM) * (1.0f / kLargest), vs = waveMax(largestR) * (1.0f / kLargest);
+      const float byM = ms > kTiny ? 1.0f / ms : 0.0f, byV = vs > kTiny ? 1.0f / vs : 0.0f;
+      uint32_t codeM = 0, codeV = 0;
+#pragma unroll
+      for (int i = 0; i < 4; ++i) {
+        const uint32_t random = randomBits(table.seed, e.random + at + i);
+        codeM |= narrowCode(fminf(fmaxf(m[i] * byM, -kLargest), kLargest), random & 0xffffu) << (8 * i);
+        codeV |= narrowCode(fminf(r[i] * byV, kLargest), random >> 16) << (8 * i);
+      }
+      if (n) {
+        storeCodes(static_cast<uint8_t*>(e.m) + at, n, codeM);
+        storeCodes(static_cast<uint8_t*>(e.v) + at, n, codeV);
+      }
+      if (threadIdx.x % 64 == 0) {
+        e.mScale[block] = ms;
+        e.vScale[block] = vs;
+      }
+    } else {
+      store4<TypeF32>(static_cast<float*>(e.m) + at, n, m);
+      store4<TypeF32>(static_cast<float*>(e.v) + at, n, v);
+    }
+  }
+}
+
+using Kernel = void (*)(Table);
+template <typename P, typename G> Kernel pick(bool small) {
+  return small ? adamwKernel<P, G, true> : adamwKernel<P, G, false>;
+}
+template <typename P> Kernel pick(int gradType, bool small) {
+  return gradType == POLAR_HIP_F32 ? pick<P, TypeF32>(small)
+         : gradType == POLAR_HIP_F16 ? pick<P, TypeF16>(small)
+                                     : pick<P, TypeBF16>(small);
+}
+
+} // namespace
+
+extern "C" {
+
+int polar_hip_fadamw(polar_hip_device* dev, const polar_hip_adamw_config* config, const polar_hip_adamw_tensor* tensors,
+                     uint64_t count) {
+  POLAR_HIP_REQUIRE(dev != nullptr && config != nullptr, "null argument");
+  POLAR_HIP_REQUIRE(count == 0 || tensors != nullptr, "null list of tensors");
+  POLAR_HIP_REQUIRE(knownType(config->param_type) && knownType(config->grad_type), "unknown element type");
+  POLAR_HIP_REQUIRE(config->state_bits == 32 || config->state_bits == 8, "states are held in 32 or 8 bits");
+  POLAR_HIP_REQUIRE(config->step >= 1, "steps are counted from 1");
+  POLAR_HIP_REQUIRE(config->beta1 >= 0 && config->beta1 < 1 && config->beta2 >= 0 && config->beta2 < 1,
+                    "beta1 and beta2 lie in [0, 1)");
+  POLAR_HIP_REQUIRE(std::isfinite(config->lr) && config->eps >= 0 && std::isfinite(config->eps) &&
+                        std::isfinite(config->grad_scale),
+                    "lr, eps and grad_scale must be finite, eps not negative");
+  const bool small = config->state_bits == 8, copy = config->param_type != POLAR_HIP_F32;
+  // everything is checked before the first tensor is touched
+  for (uint64_t i = 0; i < count; ++i) {
+    const polar_hip_adamw_tensor& t = tensors[i];
+    POLAR_HIP_REQUIRE(std::isfinite(t.weight_decay), "a tensor's weight decay is not finite");
+    if (t.count == 0) continue;
+    POLAR_HIP_REQUIRE(t.count < (1ull << 42), "a tensor is too large");
+    POLAR_HIP_REQUIRE(t.param && t.grad && t.m && t.v, "a tensor's pointer is null");
+    POLAR_HIP_REQUIRE(!copy || t.master, "16-bit parameters need an fp32 master");
+    POLAR_HIP_REQUIRE(!small || (t.m_scale && t.v_scale), "8-bit states need scales");
+    POLAR_HIP_REQUIRE(alignedTo(t.param, sizeOf(config->param_type)) && alignedTo(t.grad, sizeOf(config->grad_type)) &&
+                          (!copy || alignedTo(t.master, 4)) && (small || (alignedTo(t.m, 4) && alignedTo(t.v, 4))) &&
+                          (!small || (alignedTo(t.m_scale, 4) && alignedTo(t.v_scale, 4))),
+                      "misaligned pointer");
+  }
+  POLAR_HIP_TRY(hipSetDevice(dev->ordinal));
+  Table table{};
+  const double correction1 = 1.0 - std::pow(config->beta1, static_cast<double>(config->step));
+  const double correction2 = 1.0 - std::pow(config->beta2, static_cast<double>(config->step));
+  table.gradScale = static_cast<float>(config->grad_scale);
+  table.beta1 = static_cast<float>(config->beta1);
+  table.rest1 = static_cast<float>(1.0 - config->beta1);
+  table.beta2 = static_cast<float>(config->beta2);
+  table.rest2 = static_cast<float>(1.0 - config->beta2);
+  table.stepSize = static_cast<float>(config->lr / correction1);
+  table.byCorrection = static_cast<float>(1.0 / std::sqrt(correction2));
+  table.eps = static_cast<float>(config->eps);
+  table.seed = config->seed;
+  const Kernel kernel = config->param_type == POLAR_HIP_F32   ? pick<TypeF32>(config->grad_type, small)
+                        : config->param_type == POLAR_HIP_F16 ? pick<TypeF16>(config->grad_type, small)
+                                                              : pick<TypeBF16>(config->grad_type, small);
+  constexpr uint64_t kMostGroups = 1ull << 30; // of a launch
+  uint64_t groups = 0;
+  int listed = 0;
+  auto flush = [&]() -> int {
+    if (listed == 0) return POLAR_HIP_OK;
+    for (; listed < kTensors; ++listed) table.firstGroup[listed] = 0xffffffffu;
+    POLAR_HIP_TRY(launchKernel(dev, kernel, dim3(static_cast<unsigned>(groups)), dim3(kBlock), table));
+    listed = 0;
+    groups = 0;
+    return POLAR_HIP_OK;
+  };
+  for (uint64_t i = 0; i < count; ++i) {
+    const polar_hip_adamw_tensor& t = tensors[i];
+    if (t.count == 0) continue;
+    const uint64_t mine = (t.count + kChunk - 1) / kChunk; // below 2^30
+    if (listed == kTensors || groups + mine > kMostGroups) {
+      const int st = flush();
+      if (st != POLAR_HIP_OK) return st;
+    }
+    table.firstGroup[listed] = static_cast<uint32_t>(groups);
+    table.e[listed++] = Entry{t.param, const_cast<void*>(t.grad), t.m, t.v, t.master, t.m_scale, t.v_scale, t.count,
+                              t.first, static_cast<float>(config->lr * t.weight_decay)};
+    groups += mine;
+  }
+  return flush();
+}
+
+} // extern "C"
