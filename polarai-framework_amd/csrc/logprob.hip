@@ -5,17 +5,23 @@
 //   logprob = z_t - logsum,   entropy = logsum - S1 / S0
 //   dx_j = s (g (1[j = t] - p_j) - h p_j (ln p_j + entropy)),   p_j = e^(z_j - logsum)
 //
-// The forward pass reads the logits once.  Each lane keeps a running maximum
-// and both sums relative to it, in base 2, and rescales the sums once per tile
-// of up to 32 logits; lanes, waves and parts of a row are joined the same way.
+// The forward pass reads the logits once.  A wave keeps one reference for its
+// exponentials, the largest logit seen when it was last set, and sets it anew
+// only when a logit exceeds it by 2^64 in the exponential: sums in fp32 have
+// the room, and a tile of up to 32 logits per lane costs one comparison instead
+// of a rescaling.  Lanes, waves and parts of a row are joined relative to the
+// true maximum.
+//
 // Alternatives cost next to nothing while the row streams by: a lane notes the
 // maximum of each of its tiles (a "segment") in LDS.  The k-th best of the
-// lanes' maxima bounds the k-th best logit from below; only segments that reach
-// the bound are looked at again, the k best of them are kept, and the k best
-// logits lie in those.  Logits are compared as (value, place) with the lowest
-// place first, an order without ties, so each list has a fixed bound whatever
-// the data (a wave contributes at most k lanes, a lane 16 segments, a segment
-// 32 logits) and the answer is the same on every run.
+// lanes' maxima bounds the k-th best logit from below, and only segments that
+// reach the bound are looked at again: k of them and a few more.  Logits are
+// compared as (value, place) with the lowest place first, an order without
+// ties.  Where equal logits are so many that the bound leaves a long list
+// (constant rows, rows with fewer than k logits that are not -infinity), the
+// lanes' and then the segments' maxima are ordered by place as well, which
+// bounds every list whatever the data: k lanes per wave, 16 segments per lane,
+// then k segments of 32 logits.  The answer is the same on every run.
 #include "typed.h"
 
 #include <algorithm>
@@ -30,7 +36,8 @@ constexpr int kWaves = kBlock / 64;
 constexpr int kPacks = 4;        // 16-byte packs a lane takes per tile
 constexpr int kMaxTiles = 16;    // tiles of a part, so segments per lane
 constexpr int kMaxTop = 32;
-constexpr int kMaxListed = kWaves * kMaxTop * kMaxTiles;  // segments that can reach the bound
+constexpr int kMaxListed = kWaves * kMaxTop * kMaxTiles;  // segments that can reach the exact bound
+constexpr uint32_t kShortList = 64;                       // segments whose logits are looked at without ordering them first
 constexpr uint64_t kMaxCols = 1ull << 24;                 // places are exact as fp32 tokens
 constexpr float kLog2e = 1.44269504088896340736f;
 constexpr float kLn2 = 0.69314718055994530942f;
@@ -83,9 +90,53 @@ __device__ __forceinline__ void rankKeys(const uint64_t* keys, uint32_t count, u
   for (uint32_t e = threadIdx.x; e < count; e += kBlock) {
     const uint64_t mine = keys[e];
     uint32_t above = 0;
+#pragma unroll 8
     for (uint32_t i = 0; i < count; ++i) above += keys[i] > mine;
     if (above < wanted) emit(above, mine, e);
   }
+}
+
+// A lower bound, as an order number, of the `wanted`-th best of the work-group's
+// values: the wanted-th best of the lanes' own best (`order`, 0 for a lane without
+// any).  Six low bits give way to the lane's number so that no two lanes of a wave
+// tie: 16-bit types do not use them, in fp32 the bound is 64 units in the last
+// place lower at most.  The lanes' rank within the wave is counted through scalar
+// registers; the four waves' sorted lists are merged by binary search.
+struct BoundScratch {
+  uint32_t sorted[kWaves][kMaxTop];
+  uint32_t bound;
+};
+__device__ __forceinline__ uint32_t laneBound(uint32_t order, uint32_t wanted, BoundScratch& lds) {
+  const uint32_t lane = threadIdx.x % 64, wave = threadIdx.x / 64;
+  const uint32_t mine = (order & ~63u) | (63u - lane);
+  uint32_t rank = 0;
+#pragma unroll
+  for (int i = 0; i < 64; ++i) rank += static_cast<uint32_t>(__builtin_amdgcn_readlane(static_cast<int>(mine), i)) > mine;
+  if (rank < wanted) lds.sorted[wave][rank] = mine;
+  __syncthreads();
+  if (threadIdx.x < kWaves * kMaxTop) {
+    const uint32_t w = threadIdx.x / kMaxTop, at = threadIdx.x % kMaxTop;
+    if (at < wanted) {
+      const uint32_t key = lds.sorted[w][at];
+      uint32_t above = at;
+#pragma unroll
+      for (uint32_t o = 0; o < kWaves; ++o) {
+        if (o == w) continue;
+        // entries of wave o in front of this one: larger, or equal and of an earlier wave
+        uint32_t low = 0;
+#pragma unroll
+        for (uint32_t half = kMaxTop; half > 0; half /= 2) {
+          const uint32_t probe = low + half - 1;
+          const bool front = probe < wanted && (lds.sorted[o][probe % kMaxTop] > key || (o < w && lds.sorted[o][probe % kMaxTop] == key));
+          if (front) low += half;
+        }
+        above += low;
+      }
+      if (above == wanted - 1) lds.bound = key & ~63u;
+    }
+  }
+  __syncthreads();
+  return lds.bound;
 }
 
 struct ForwardArgs {
@@ -104,10 +155,23 @@ struct ForwardArgs {
   uint64_t* partKeys;
 };
 
+// A row's given token and its logit, loaded by one lane before the row streams by.
+struct Given {
+  int64_t token;
+  float logit;
+};
+template <typename T> __device__ __forceinline__ Given givenOf(const ForwardArgs& a, uint64_t row) {
+  Given g{-1, 0.0f};
+  if (threadIdx.x == 0 && a.logprob != nullptr) {
+    g.token = tokenAt(a.tokens, a.tokenType, row);
+    if (g.token >= 0 && g.token < int64_t(a.cols))
+      g.logit = T::widen((static_cast<const typename T::Stored*>(a.logits) + row * a.stride)[g.token]);
+  }
+  return g;
+}
+
 // The row's answers, from its joined sums and its best keys in LDS.
-template <typename T>
-__device__ __forceinline__ void finishRow(const ForwardArgs& a, uint64_t row, RowSums r, const uint64_t* best) {
-  const typename T::Stored* x = static_cast<const typename T::Stored*>(a.logits) + row * a.stride;
+__device__ __forceinline__ void finishRow(const ForwardArgs& a, uint64_t row, Given given, RowSums r, const uint64_t* best) {
   const float logsum = logf(r.s0); // -infinity where every logit is
   const bool none = r.s0 == 0.0f;
   if (threadIdx.x == 0) {
@@ -117,12 +181,11 @@ __device__ __forceinline__ void finishRow(const ForwardArgs& a, uint64_t row, Ro
     }
     if (a.entropy != nullptr) a.entropy[row] = none ? 0.0f : kLn2 * (log2f(r.s0) - r.s1 / r.s0);
     if (a.logprob != nullptr) {
-      const int64_t t = tokenAt(a.tokens, a.tokenType, row);
       float lp = 0.0f;
-      if (t >= int64_t(a.cols))
+      if (given.token >= int64_t(a.cols))
         lp = __builtin_nanf("");
-      else if (t >= 0)
-        lp = none ? -__builtin_inff() : (T::widen(x[t]) - r.m) * a.scale - logsum;
+      else if (given.token >= 0)
+        lp = none ? -__builtin_inff() : (given.logit - r.m) * a.scale - logsum;
       a.logprob[row] = lp;
     }
   }
@@ -139,10 +202,12 @@ __device__ __forceinline__ void finishRow(const ForwardArgs& a, uint64_t row, Ro
 template <typename T, bool kEntropy, bool kTop>
 __global__ __launch_bounds__(kBlock) void logprobKernel(ForwardArgs a) {
   constexpr int kVec = T::kVec;
+  constexpr int kLane = kPacks * kVec; // logits of a lane per tile
   constexpr uint32_t kTile = tileCols<T>();
   using Stored = typename T::Stored;
   __shared__ RowSums waveSums[kWaves];
   __shared__ uint64_t waveBound[kWaves];
+  __shared__ BoundScratch scratch;
   __shared__ uint32_t listed, found;
   // segment maxima while the row streams by, then the listed segments' keys, then the logits' keys
   __shared__ __align__(16) unsigned char area[kTop ? kMaxListed * sizeof(uint64_t) : 16];
@@ -150,7 +215,7 @@ __global__ __launch_bounds__(kBlock) void logprobKernel(ForwardArgs a) {
   __shared__ uint16_t kept[kTop ? kMaxTop : 1];
   __shared__ uint64_t best[kTop ? kMaxTop : 1];
   static_assert(kMaxListed * sizeof(uint64_t) >= kMaxTiles * kBlock * sizeof(float), "segment maxima fit");
-  static_assert(kMaxListed >= kMaxTop * kPacks * 8, "the kept segments' logits fit");
+  static_assert(kMaxListed >= kShortList * 4 * 8 && kMaxListed >= kMaxTop * 4 * 8, "the looked-at segments' logits fit");
 
   const uint64_t row = a.firstRow + blockIdx.x / a.parts;
   const uint32_t part = blockIdx.x % a.parts;
@@ -161,17 +226,28 @@ __global__ __launch_bounds__(kBlock) void logprobKernel(ForwardArgs a) {
   const float c = a.scale * kLog2e;
   const Stored kNothing = static_cast<Stored>(-__builtin_inff());
   float* segments = reinterpret_cast<float*>(area);
+  const Given given = a.parts == 1 ? givenOf<T>(a, row) : Given{-1, 0.0f};
 
   auto place = [&](uint32_t tile, int k, uint32_t lane) { return begin + tile * kTile + (k * kBlock + lane) * kVec; };
 
-  RowSums r{-__builtin_inff(), 0.0f, 0.0f};
-  float laneBest = -__builtin_inff();
+  // the wave's reference; a lane's sums of 2^(x c + shift), whose exponents lack `rest`:
+  // the product's rounding error is the same for all of them and is put in at the end,
+  // so that logits far from zero lose nothing against (x - reference) c
+  float reference = -__builtin_inff(), limit = -__builtin_inff(), shift = 0.0f, rest = 0.0f;
+  bool wide = false, masked = false; // of the whole wave
+  float laneBest = -__builtin_inff(), s0 = 0.0f, s1 = 0.0f;
   uint32_t laneTile = 0;
+  auto settle = [&](float to) { // sums relative to `to`
+    if constexpr (kEntropy) s1 += rest * s0;
+    const float d = rebase(reference, to, c), f = __builtin_amdgcn_exp2f(d + rest);
+    if constexpr (kEntropy) s1 = (s1 + s0 * d) * f;
+    s0 *= f;
+  };
   Pack next[kPacks];
 #pragma unroll
   for (int k = 0; k < kPacks; ++k) next[k] = loadPack<T, false>(x, place(0, k, threadIdx.x), end, kNothing);
   for (uint32_t tile = 0; tile < tiles; ++tile) {
-    float v[kPacks * kVec];
+    float v[kLane];
 #pragma unroll
     for (int k = 0; k < kPacks; ++k) T::unpack(next[k], v + k * kVec);
     if (tile + 1 < tiles) {
@@ -180,129 +256,156 @@ __global__ __launch_bounds__(kBlock) void logprobKernel(ForwardArgs a) {
     }
     float most = v[0];
 #pragma unroll
-    for (int i = 1; i < kPacks * kVec; ++i) most = fmaxf(most, v[i]);
+    for (int i = 1; i < kLane; ++i) most = fmaxf(most, v[i]);
     if constexpr (kTop) {
-      segments[tile * kBlock + threadIdx.x] = most;
-      if (most > laneBest) laneBest = most, laneTile = tile;
+      // a lane whose segment lies behind the end has none
+      segments[tile * kBlock + threadIdx.x] = place(tile, 0, threadIdx.x) < end ? most : __builtin_nanf("");
+      if (most > laneBest) laneTile = tile;
     }
-    const float m = fmaxf(r.m, most);
-    const float base = m == -__builtin_inff() ? 0.0f : m;
-    // y = x c - base c as one fused multiply-add; the rounding error of base c is
-    // the same for the whole tile and is taken out of its sums afterwards, so
-    // that logits far from zero lose nothing against (x - base) c
-    const float shift = -base * c;
-    const float rest = __builtin_fmaf(-base, c, -shift);
-    float t0 = 0.0f, t1 = 0.0f, off = rest;
-    if (__any(fabsf(base) > 1e30f)) { // base c might overflow (a row masked with the type's lowest value)
+    laneBest = fmaxf(laneBest, most);
+    if (__any(most > limit)) {
+      const float to = waveMax(laneBest);
+      settle(to);
+      reference = to;
+      limit = to + 64.0f / c;
+      wide = fabsf(to) > 1e30f; // to * c might overflow: a row masked with the type's lowest value
+      shift = wide ? 0.0f : -to * c;
+      rest = wide ? 0.0f : __builtin_fmaf(-to, c, -shift);
+    }
+    float t1 = 0.0f;
+    if (wide) {
 #pragma unroll
-      for (int i = 0; i < kPacks * kVec; ++i) {
-        const float y = (v[i] - base) * c;
-        const float e = __builtin_amdgcn_exp2f(y);
-        t0 += e;
+      for (int i = 0; i < kLane; ++i) {
+        const float y = (v[i] - reference) * c, e = __builtin_amdgcn_exp2f(y);
+        s0 += e;
         if constexpr (kEntropy) t1 = __builtin_fmaf(e, fmaxf(y, -160.0f), t1);
       }
-      off = 0.0f;
+    } else if (kEntropy && masked) {
+#pragma unroll
+      for (int i = 0; i < kLane; ++i) {
+        const float y = __builtin_fmaf(v[i], c, shift), e = __builtin_amdgcn_exp2f(y);
+        s0 += e;
+        t1 = __builtin_fmaf(e, fmaxf(y, -160.0f), t1);
+      }
     } else {
 #pragma unroll
-      for (int i = 0; i < kPacks * kVec; ++i) {
-        const float y = __builtin_fmaf(v[i], c, shift);
-        const float e = __builtin_amdgcn_exp2f(y); // 0 below 2^-149, NaN for NaN
-        t0 += e;
-        if constexpr (kEntropy) t1 = __builtin_fmaf(e, fmaxf(y, -160.0f), t1); // 0 * -infinity is no term
+      for (int i = 0; i < kLane; ++i) {
+        const float y = __builtin_fmaf(v[i], c, shift), e = __builtin_amdgcn_exp2f(y); // 0 below 2^-149, NaN for NaN
+        s0 += e;
+        if constexpr (kEntropy) t1 = __builtin_fmaf(e, y, t1);
+      }
+      if constexpr (kEntropy) {
+        // 0 * -infinity is no term: from the first one on the wave clamps its exponents
+        masked = __any(t1 != t1);
+        if (masked) {
+          t1 = 0.0f;
+#pragma unroll
+          for (int i = 0; i < kLane; ++i) {
+            const float y = __builtin_fmaf(v[i], c, shift);
+            t1 = __builtin_fmaf(__builtin_amdgcn_exp2f(y), fmaxf(y, -160.0f), t1);
+          }
+        }
       }
     }
-    const float d = rebase(r.m, m, c), f = __builtin_amdgcn_exp2f(d), g = __builtin_amdgcn_exp2f(off);
-    if constexpr (kEntropy) r.s1 = (r.s1 + r.s0 * d) * f + (t1 + off * t0) * g;
-    r.s0 = r.s0 * f + t0 * g;
-    r.m = m;
+    if constexpr (kEntropy) s1 += t1;
   }
 
   // lanes, then waves
   {
-    const float m = waveMax(r.m);
-    const float d = rebase(r.m, m, c), f = __builtin_amdgcn_exp2f(d);
-    const float s1 = kEntropy ? waveSum((r.s1 + r.s0 * d) * f) : 0.0f;
-    const float s0 = waveSum(r.s0 * f);
-    if (threadIdx.x % 64 == 0) waveSums[threadIdx.x / 64] = RowSums{m, s0, s1};
+    const float m = waveMax(laneBest);
+    settle(m);
+    const float sum1 = kEntropy ? waveSum(s1) : 0.0f, sum0 = waveSum(s0);
+    if (threadIdx.x % 64 == 0) waveSums[threadIdx.x / 64] = RowSums{m, sum0, sum1};
   }
 
   if constexpr (kTop) {
-    // first place of a segment's maximum
-    auto segmentKey = [&](uint32_t tile, uint32_t lane, float most) {
-      uint32_t at = 0xffffffffu;
-#pragma unroll
-      for (int k = kPacks - 1; k >= 0; --k) {
-        float w[kVec];
-        T::unpack(loadPack<T, false>(x, place(tile, k, lane), end, kNothing), w);
-#pragma unroll
-        for (int i = kVec - 1; i >= 0; --i) {
-          const uint32_t p = place(tile, k, lane) + i;
-          if (p < end && w[i] == most) at = p;
-        }
-      }
-      return at == 0xffffffffu ? 0ull : keyOf(most, at);
-    };
-    // the wave's k-th best lane: a bitonic network over the 64 lanes' best keys
-    const uint32_t lane = threadIdx.x % 64;
-    const uint64_t laneKey = segmentKey(laneTile, threadIdx.x, laneBest);
-    uint64_t sorted = laneKey;
-#pragma unroll
-    for (uint32_t size = 2; size <= 64; size *= 2) {
-#pragma unroll
-      for (uint32_t gap = size / 2; gap > 0; gap /= 2) {
-        const uint64_t other = __shfl_xor(sorted, gap, 64);
-        const bool larger = ((lane & size) == 0) == ((lane & gap) == 0); // descending over the whole wave
-        sorted = (other > sorted) == larger ? other : sorted;
-      }
-    }
-    const uint64_t bound1 = __shfl(sorted, a.top - 1, 64);
-    if (lane == 0) waveBound[threadIdx.x / 64] = bound1;
-    if (threadIdx.x == 0) listed = found = 0;
-    __syncthreads();
-    uint64_t bound = waveBound[0];
-#pragma unroll
-    for (int w = 1; w < kWaves; ++w) bound = bound > waveBound[w] ? bound : waveBound[w];
-    // segments that reach the bound (by their value: the places come next)
-    if (laneKey != 0 && laneKey >= bound) {
-      const uint32_t least = static_cast<uint32_t>(bound >> 32);
-      for (uint32_t tile = 0; tile < tiles; ++tile)
-        if (orderOf(segments[tile * kBlock + threadIdx.x]) >= least)
-          list[atomicAdd(&listed, 1u)] = static_cast<uint16_t>(tile * kBlock + threadIdx.x);
-    }
-    __syncthreads(); // the list is whole, and the maxima are not needed any more
-    const uint32_t count = listed;
     uint64_t* keys = reinterpret_cast<uint64_t*>(area);
-    uint32_t keep = count;
-    if (count > a.top) {
-      keep = a.top;
-      for (uint32_t e = threadIdx.x; e < count; e += kBlock) {
-        const uint32_t tile = list[e] / kBlock, owner = list[e] % kBlock;
-        float most = -__builtin_inff();
-#pragma unroll
-        for (int k = 0; k < kPacks; ++k) {
-          float w[kVec];
-          T::unpack(loadPack<T, false>(x, place(tile, k, owner), end, kNothing), w);
-#pragma unroll
-          for (int i = 0; i < kVec; ++i) most = fmaxf(most, w[i]);
+    const bool some = place(0, 0, threadIdx.x) < end;
+    if (threadIdx.x == 0) listed = found = 0;
+    const uint32_t least = laneBound(some ? orderOf(laneBest) : 0u, a.top, scratch);
+    auto listSegments = [&](uint32_t from) { // those whose maximum's order is not below `from`
+      for (uint32_t tile = 0; tile < tiles; ++tile) {
+        const uint32_t order = orderOf(segments[tile * kBlock + threadIdx.x]);
+        if (order >= from && order != 0) {
+          const uint32_t at = atomicAdd(&listed, 1u);
+          if (at < kMaxListed) list[at] = static_cast<uint16_t>(tile * kBlock + threadIdx.x);
         }
-        // a segment without a valid logit has key 0: distinct below all others is all that rank needs
-        const uint64_t key = segmentKey(tile, owner, most);
-        keys[e] = key != 0 ? key : e;
       }
-      if (threadIdx.x < kMaxTop) best[threadIdx.x] = 0;
+    };
+    if (orderOf(laneBest) >= least) listSegments(least);
+    __syncthreads();
+    uint64_t bound = uint64_t(least) << 32; // of the logits' keys
+    const uint16_t* looked = list;
+    uint32_t count = listed;
+    if (count > kShortList) { // uniform
+      // first place of a segment's maximum
+      auto segmentKey = [&](uint32_t tile, uint32_t lane, float most) {
+        uint32_t at = 0xffffffffu;
+#pragma unroll
+        for (int k = kPacks - 1; k >= 0; --k) {
+          float w[kVec];
+          T::unpack(loadPack<T, false>(x, place(tile, k, lane), end, kNothing), w);
+#pragma unroll
+          for (int i = kVec - 1; i >= 0; --i) {
+            const uint32_t p = place(tile, k, lane) + i;
+            if (p < end && w[i] == most) at = p;
+          }
+        }
+        return at == 0xffffffffu ? 0ull : keyOf(most, at);
+      };
+      // the wave's k-th best lane: a bitonic network over the 64 lanes' best keys
+      const uint32_t lane = threadIdx.x % 64;
+      const uint64_t laneKey = segmentKey(laneTile, threadIdx.x, laneBest);
+      uint64_t sorted = laneKey;
+#pragma unroll
+      for (uint32_t size = 2; size <= 64; size *= 2) {
+#pragma unroll
+        for (uint32_t gap = size / 2; gap > 0; gap /= 2) {
+          const uint64_t other = __shfl_xor(sorted, gap, 64);
+          const bool larger = ((lane & size) == 0) == ((lane & gap) == 0); // descending over the whole wave
+          sorted = (other > sorted) == larger ? other : sorted;
+        }
+      }
+      const uint64_t bound1 = __shfl(sorted, a.top - 1, 64);
+      if (lane == 0) waveBound[threadIdx.x / 64] = bound1;
+      __syncthreads(); // everyone has read the first list's length
+      if (threadIdx.x == 0) listed = 0;
       __syncthreads();
-      rankKeys(keys, count, a.top, [&](uint32_t rank, uint64_t key, uint32_t e) {
-        kept[rank] = list[e];
-        best[rank] = key;
-      });
-      __syncthreads(); // also: the segments' keys are read
-      bound = bound > best[a.top - 1] ? bound : best[a.top - 1];
-    } else {
-      if (threadIdx.x < count) kept[threadIdx.x] = list[threadIdx.x];
-      __syncthreads();
+      bound = waveBound[0];
+#pragma unroll
+      for (int w = 1; w < kWaves; ++w) bound = bound > waveBound[w] ? bound : waveBound[w];
+      // of at most k lanes per wave the segments that may reach the bound: at most kMaxListed
+      if (laneKey != 0 && laneKey >= bound) listSegments(static_cast<uint32_t>(bound >> 32));
+      __syncthreads(); // the list is whole, and the maxima are not needed any more
+      count = listed;
+      if (count > a.top) {
+        for (uint32_t e = threadIdx.x; e < count; e += kBlock) {
+          const uint32_t tile = list[e] / kBlock, owner = list[e] % kBlock;
+          float most = -__builtin_inff();
+#pragma unroll
+          for (int k = 0; k < kPacks; ++k) {
+            float w[kVec];
+            T::unpack(loadPack<T, false>(x, place(tile, k, owner), end, kNothing), w);
+#pragma unroll
+            for (int i = 0; i < kVec; ++i) most = fmaxf(most, w[i]);
+          }
+          // without a logit: a key below all others, and no two alike
+          const uint64_t key = segmentKey(tile, owner, most);
+          keys[e] = key != 0 ? key : e;
+        }
+        __syncthreads();
+        rankKeys(keys, count, a.top, [&](uint32_t rank, uint64_t key, uint32_t e) {
+          kept[rank] = list[e];
+          best[rank] = key;
+        });
+        __syncthreads(); // also: the segments' keys are read
+        bound = bound > best[a.top - 1] ? bound : best[a.top - 1];
+        count = a.top;
+        looked = kept;
+      }
     }
-    for (uint32_t e = threadIdx.x; e < keep * kPacks; e += kBlock) {
-      const uint32_t segment = kept[e / kPacks];
+    for (uint32_t e = threadIdx.x; e < count * kPacks; e += kBlock) {
+      const uint32_t segment = looked[e / kPacks];
       const uint32_t from = place(segment / kBlock, e % kPacks, segment % kBlock);
       float w[kVec];
       T::unpack(loadPack<T, false>(x, from, end, kNothing), w);
@@ -321,7 +424,7 @@ __global__ __launch_bounds__(kBlock) void logprobKernel(ForwardArgs a) {
 #pragma unroll
   for (int w = 1; w < kWaves; ++w) total = join(total, waveSums[w], c);
   if (a.parts == 1) {
-    finishRow<T>(a, row, total, best);
+    finishRow(a, row, given, total, best);
   } else {
     const uint64_t slot = uint64_t(blockIdx.x);
     if (threadIdx.x == 0) a.partSums[slot] = total;
@@ -329,36 +432,65 @@ __global__ __launch_bounds__(kBlock) void logprobKernel(ForwardArgs a) {
   }
 }
 
-// Joins the parts of a row: one work-group per row, in the order of the parts.
+// Joins the parts of a row: one work-group per row.  The sums: a lane per part,
+// in the first wave.  The keys: those that reach the bound that the lanes' best
+// ones give, ranked; where they are too many (logits that are equal all over
+// the row), stretches of the keys are ranked together with the best so far.
 constexpr uint32_t kJoinKeys = 2048;
 template <typename T>
 __global__ __launch_bounds__(kBlock) void logprobJoinKernel(ForwardArgs a) {
   __shared__ uint64_t keys[kJoinKeys];
   __shared__ uint64_t best[kMaxTop];
-  const uint64_t slot = uint64_t(blockIdx.x) * a.parts;
+  __shared__ BoundScratch scratch;
+  __shared__ RowSums sums;
+  __shared__ uint32_t listed;
+  const uint64_t row = a.firstRow + blockIdx.x, slot = uint64_t(blockIdx.x) * a.parts;
   const float c = a.scale * kLog2e;
-  RowSums r = a.partSums[slot];
-  for (uint32_t p = 1; p < a.parts; ++p) r = join(r, a.partSums[slot + p], c);
+  const Given given = givenOf<T>(a, row);
+  if (threadIdx.x < 64) {
+    RowSums r{-__builtin_inff(), 0.0f, 0.0f};
+    for (uint32_t p = threadIdx.x; p < a.parts; p += 64) r = join(r, a.partSums[slot + p], c);
+    const float m = waveMax(r.m);
+    const float d = rebase(r.m, m, c), f = __builtin_amdgcn_exp2f(d);
+    const float s1 = waveSum((r.s1 + r.s0 * d) * f), s0 = waveSum(r.s0 * f);
+    if (threadIdx.x == 0) sums = RowSums{m, s0, s1};
+  }
   if (a.top != 0) {
     const uint64_t* from = a.partKeys + slot * a.top;
     const uint32_t all = a.parts * a.top;
-    if (threadIdx.x < kMaxTop) best[threadIdx.x] = 0;
-    for (uint32_t at = 0; at < all; at += kJoinKeys - kMaxTop) { // and the best so far
-      const uint32_t count = all - at < kJoinKeys - kMaxTop ? all - at : kJoinKeys - kMaxTop;
-      __syncthreads();
-      for (uint32_t e = threadIdx.x; e < count; e += kBlock) keys[e] = from[at + e];
-      if (threadIdx.x < a.top) keys[count + threadIdx.x] = best[threadIdx.x];
-      __syncthreads();
-      if (threadIdx.x < kMaxTop) best[threadIdx.x] = 0;
-      __syncthreads();
-      // empty places (key 0) are not distinct, but rank below every logit: they emit zeros
-      rankKeys(keys, count + a.top, a.top, [&](uint32_t rank, uint64_t key, uint32_t) {
-        if (key != 0) best[rank] = key;
-      });
+    uint64_t mine = 0;
+    for (uint32_t e = threadIdx.x; e < all; e += kBlock) mine = from[e] > mine ? from[e] : mine;
+    if (threadIdx.x == 0) listed = 0;
+    const uint32_t least = laneBound(static_cast<uint32_t>(mine >> 32), a.top, scratch);
+    for (uint32_t e = threadIdx.x; e < all; e += kBlock) {
+      const uint64_t key = from[e];
+      if (key != 0 && static_cast<uint32_t>(key >> 32) >= least) {
+        const uint32_t at = atomicAdd(&listed, 1u);
+        if (at < kJoinKeys) keys[at] = key;
+      }
     }
+    if (threadIdx.x < kMaxTop) best[threadIdx.x] = 0;
     __syncthreads();
+    if (listed <= kJoinKeys) { // uniform
+      rankKeys(keys, listed, a.top, [&](uint32_t rank, uint64_t key, uint32_t) { best[rank] = key; });
+    } else {
+      for (uint32_t at = 0; at < all; at += kJoinKeys - kMaxTop) {
+        const uint32_t count = all - at < kJoinKeys - kMaxTop ? all - at : kJoinKeys - kMaxTop;
+        __syncthreads();
+        for (uint32_t e = threadIdx.x; e < count; e += kBlock) keys[e] = from[at + e];
+        if (threadIdx.x < a.top) keys[count + threadIdx.x] = best[threadIdx.x];
+        __syncthreads();
+        if (threadIdx.x < kMaxTop) best[threadIdx.x] = 0;
+        __syncthreads();
+        // empty places (key 0) are not distinct, but rank below every logit
+        rankKeys(keys, count + a.top, a.top, [&](uint32_t rank, uint64_t key, uint32_t) {
+          if (key != 0) best[rank] = key;
+        });
+      }
+    }
   }
-  finishRow<T>(a, a.firstRow + blockIdx.x, r, best);
+  __syncthreads();
+  finishRow(a, row, given, sums, best);
 }
 
 // ---- gradient ----------------------------------------------------------------------
