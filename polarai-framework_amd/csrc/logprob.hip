@@ -38,6 +38,7 @@ constexpr int kMaxTiles = 16;    // tiles of a part, so segments per lane
 constexpr int kMaxTop = 32;
 constexpr int kMaxListed = kWaves * kMaxTop * kMaxTiles;  // segments that can reach the exact bound
 constexpr uint32_t kShortList = 64;                       // segments whose logits are looked at without ordering them first
+constexpr uint32_t kStagedAt = 12288;                     // bytes in front of the staged packs of a part of one tile
 constexpr uint64_t kMaxCols = 1ull << 24;                 // places are exact as fp32 tokens
 constexpr float kLog2e = 1.44269504088896340736f;
 constexpr float kLn2 = 0.69314718055994530942f;
@@ -90,50 +91,38 @@ __device__ __forceinline__ void rankKeys(const uint64_t* keys, uint32_t count, u
   for (uint32_t e = threadIdx.x; e < count; e += kBlock) {
     const uint64_t mine = keys[e];
     uint32_t above = 0;
-#pragma unroll 8
+#pragma unroll 4
     for (uint32_t i = 0; i < count; ++i) above += keys[i] > mine;
     if (above < wanted) emit(above, mine, e);
   }
 }
 
 // A lower bound, as an order number, of the `wanted`-th best of the work-group's
-// values: the wanted-th best of the lanes' own best (`order`, 0 for a lane without
-// any).  Six low bits give way to the lane's number so that no two lanes of a wave
-// tie: 16-bit types do not use them, in fp32 the bound is 64 units in the last
-// place lower at most.  The lanes' rank within the wave is counted through scalar
-// registers; the four waves' sorted lists are merged by binary search.
+// values: the wanted-th best of its lanes' own best (`order`; 0 for a lane without
+// any), with the bits behind the first kBits cleared.  The first wave finds it bit
+// by bit, counting with ballots the lanes that reach a candidate: compares are its
+// only vector instructions, the rest is scalar.
 struct BoundScratch {
-  uint32_t sorted[kWaves][kMaxTop];
+  uint32_t lanes[kBlock];
   uint32_t bound;
 };
-__device__ __forceinline__ uint32_t laneBound(uint32_t order, uint32_t wanted, BoundScratch& lds) {
-  const uint32_t lane = threadIdx.x % 64, wave = threadIdx.x / 64;
-  const uint32_t mine = (order & ~63u) | (63u - lane);
-  uint32_t rank = 0;
-#pragma unroll
-  for (int i = 0; i < 64; ++i) rank += static_cast<uint32_t>(__builtin_amdgcn_readlane(static_cast<int>(mine), i)) > mine;
-  if (rank < wanted) lds.sorted[wave][rank] = mine;
+template <int kBits> __device__ __forceinline__ uint32_t laneBound(uint32_t order, uint32_t wanted, BoundScratch& lds) {
+  lds.lanes[threadIdx.x] = order;
   __syncthreads();
-  if (threadIdx.x < kWaves * kMaxTop) {
-    const uint32_t w = threadIdx.x / kMaxTop, at = threadIdx.x % kMaxTop;
-    if (at < wanted) {
-      const uint32_t key = lds.sorted[w][at];
-      uint32_t above = at;
+  if (threadIdx.x < 64) {
+    uint32_t mine[kWaves];
 #pragma unroll
-      for (uint32_t o = 0; o < kWaves; ++o) {
-        if (o == w) continue;
-        // entries of wave o in front of this one: larger, or equal and of an earlier wave
-        uint32_t low = 0;
+    for (int w = 0; w < kWaves; ++w) mine[w] = lds.lanes[w * 64 + threadIdx.x];
+    uint32_t bound = 0;
+#pragma unroll 1 // code that runs once per work-group is mostly waited for: short is fast
+    for (int bit = 31; bit >= 32 - kBits; --bit) {
+      const uint32_t candidate = bound | (1u << bit);
+      uint32_t reach = 0;
 #pragma unroll
-        for (uint32_t half = kMaxTop; half > 0; half /= 2) {
-          const uint32_t probe = low + half - 1;
-          const bool front = probe < wanted && (lds.sorted[o][probe % kMaxTop] > key || (o < w && lds.sorted[o][probe % kMaxTop] == key));
-          if (front) low += half;
-        }
-        above += low;
-      }
-      if (above == wanted - 1) lds.bound = key & ~63u;
+      for (int w = 0; w < kWaves; ++w) reach += __popcll(__ballot(mine[w] >= candidate));
+      bound = reach >= wanted ? candidate : bound;
     }
+    if (threadIdx.x == 0) lds.bound = bound;
   }
   __syncthreads();
   return lds.bound;
@@ -150,9 +139,11 @@ struct ForwardArgs {
   float* topLogprob;
   uint32_t top, cols, parts, tilesPerPart;
   uint64_t firstRow;
-  // parts > 1: [row][part] sums and [row][part][top] keys
-  RowSums* partSums;
-  uint64_t* partKeys;
+  // parts > 1: a slot per part, and per row how many of its work-groups have
+  // written theirs (all zero when the kernel starts)
+  unsigned char* slots;
+  uint32_t slotBytes;
+  uint32_t* arrived;
 };
 
 // A row's given token and its logit, loaded by one lane before the row streams by.
@@ -199,8 +190,81 @@ __device__ __forceinline__ void finishRow(const ForwardArgs& a, uint64_t row, Gi
   }
 }
 
+// ---- parts of a row --------------------------------------------------------------
+// The work-group that finishes its part last joins the row: no second launch.  A
+// part's answer goes into a slot of whole 128-byte lines of its own (sums, then its
+// best keys) with stores that are visible to the whole device (written through the
+// XCD's L2), is acknowledged, and only then counted.  No fence: writing back and
+// invalidating an L2 per work-group costs far more than all of this (64 rows of
+// 131072 in sixteen parts: 33 us with fences, 15 with a second kernel).
+constexpr uint32_t kSumsBytes = 16;
+template <typename V> __device__ __forceinline__ void putPart(unsigned char* at, V value) {
+  __hip_atomic_store(reinterpret_cast<V*>(at), value, __ATOMIC_RELAXED, __HIP_MEMORY_SCOPE_AGENT);
+}
+template <typename V> __device__ __forceinline__ V takePart(const unsigned char* at) {
+  return __hip_atomic_load(reinterpret_cast<const V*>(at), __ATOMIC_RELAXED, __HIP_MEMORY_SCOPE_AGENT);
+}
+
+// The row's parts joined, in every wave by itself: a lane per part.
+__device__ __forceinline__ RowSums joinSums(const unsigned char* slots, uint32_t slotBytes, uint32_t parts, float c) {
+  RowSums r{-__builtin_inff(), 0.0f, 0.0f};
+  for (uint32_t p = threadIdx.x % 64; p < parts; p += 64) {
+    const unsigned char* at = slots + uint64_t(p) * slotBytes;
+    r = join(r, RowSums{takePart<float>(at), takePart<float>(at + 4), takePart<float>(at + 8)}, c);
+  }
+  const float m = waveMax(r.m);
+  const float d = rebase(r.m, m, c), f = __builtin_amdgcn_exp2f(d);
+  return RowSums{m, waveSum(r.s0 * f), waveSum((r.s1 + r.s0 * d) * f)};
+}
+
+// The `top` best of the parts' keys (0 for none) into `best`: those that reach the
+// bound that the lanes' best ones give, ranked.  Where these are too many (logits
+// that are equal all over the row) stretches of the keys are ranked together with the
+// best so far.  `keys` has room for kJoinKeys.
+constexpr uint32_t kJoinKeys = kMaxListed;
+template <typename T>
+__device__ __forceinline__ void joinKeys(const unsigned char* slots, uint32_t slotBytes, uint32_t parts, uint32_t top,
+                                         uint64_t* keys, uint64_t* best, BoundScratch& scratch, uint32_t* listed) {
+  const uint32_t all = parts * top;
+  auto keyAt = [&](uint32_t e) {
+    return takePart<uint64_t>(slots + uint64_t(e / top) * slotBytes + kSumsBytes + e % top * sizeof(uint64_t));
+  };
+  uint64_t first = threadIdx.x < all ? keyAt(threadIdx.x) : 0, mine = first;
+  for (uint32_t e = threadIdx.x + kBlock; e < all; e += kBlock) mine = keyAt(e) > mine ? keyAt(e) : mine;
+  if (threadIdx.x == 0) *listed = 0;
+  const uint32_t least = laneBound<T::kOrderBits>(static_cast<uint32_t>(mine >> 32), top, scratch);
+  for (uint32_t e = threadIdx.x; e < all; e += kBlock) {
+    const uint64_t key = e < kBlock ? first : keyAt(e);
+    if (key != 0 && static_cast<uint32_t>(key >> 32) >= least) {
+      const uint32_t at = atomicAdd(listed, 1u);
+      if (at < kJoinKeys) keys[at] = key;
+    }
+  }
+  if (threadIdx.x < kMaxTop) best[threadIdx.x] = 0;
+  __syncthreads();
+  const uint32_t count = *listed;
+  if (count <= kJoinKeys) { // uniform
+    rankKeys(keys, count, top, [&](uint32_t rank, uint64_t key, uint32_t) { best[rank] = key; });
+  } else {
+    for (uint32_t at = 0; at < all; at += kJoinKeys - kMaxTop) {
+      const uint32_t n = all - at < kJoinKeys - kMaxTop ? all - at : kJoinKeys - kMaxTop;
+      __syncthreads();
+      for (uint32_t e = threadIdx.x; e < n; e += kBlock) keys[e] = keyAt(at + e);
+      if (threadIdx.x < top) keys[n + threadIdx.x] = best[threadIdx.x];
+      __syncthreads();
+      if (threadIdx.x < kMaxTop) best[threadIdx.x] = 0;
+      __syncthreads();
+      // empty places (key 0) are not distinct, but rank below every logit
+      rankKeys(keys, n + top, top, [&](uint32_t rank, uint64_t key, uint32_t) {
+        if (key != 0) best[rank] = key;
+      });
+    }
+  }
+  __syncthreads();
+}
+
 template <typename T, bool kEntropy, bool kTop>
-__global__ __launch_bounds__(kBlock) void logprobKernel(ForwardArgs a) {
+__global__ __launch_bounds__(kBlock, 5) void logprobKernel(ForwardArgs a) {
   constexpr int kVec = T::kVec;
   constexpr int kLane = kPacks * kVec; // logits of a lane per tile
   constexpr uint32_t kTile = tileCols<T>();
@@ -215,7 +279,8 @@ __global__ __launch_bounds__(kBlock) void logprobKernel(ForwardArgs a) {
   __shared__ uint16_t kept[kTop ? kMaxTop : 1];
   __shared__ uint64_t best[kTop ? kMaxTop : 1];
   static_assert(kMaxListed * sizeof(uint64_t) >= kMaxTiles * kBlock * sizeof(float), "segment maxima fit");
-  static_assert(kMaxListed >= kShortList * 4 * 8 && kMaxListed >= kMaxTop * 4 * 8, "the looked-at segments' logits fit");
+  static_assert(kMaxListed >= kShortList * kLane && kMaxListed >= kMaxTop * kLane, "the looked-at segments' logits fit");
+  static_assert(kStagedAt + kShortList * kPacks * sizeof(Pack) <= kMaxListed * sizeof(uint64_t), "staged packs fit");
 
   const uint64_t row = a.firstRow + blockIdx.x / a.parts;
   const uint32_t part = blockIdx.x % a.parts;
@@ -226,7 +291,7 @@ __global__ __launch_bounds__(kBlock) void logprobKernel(ForwardArgs a) {
   const float c = a.scale * kLog2e;
   const Stored kNothing = static_cast<Stored>(-__builtin_inff());
   float* segments = reinterpret_cast<float*>(area);
-  const Given given = a.parts == 1 ? givenOf<T>(a, row) : Given{-1, 0.0f};
+  const Given given = givenOf<T>(a, row); // by every part: any of them may be the last
 
   auto place = [&](uint32_t tile, int k, uint32_t lane) { return begin + tile * kTile + (k * kBlock + lane) * kVec; };
 
@@ -245,14 +310,14 @@ __global__ __launch_bounds__(kBlock) void logprobKernel(ForwardArgs a) {
   };
   Pack next[kPacks];
 #pragma unroll
-  for (int k = 0; k < kPacks; ++k) next[k] = loadPack<T, false>(x, place(0, k, threadIdx.x), end, kNothing);
+  for (int k = 0; k < kPacks; ++k) next[k] = loadPack<T>(x, place(0, k, threadIdx.x), end, kNothing);
   for (uint32_t tile = 0; tile < tiles; ++tile) {
     float v[kLane];
 #pragma unroll
     for (int k = 0; k < kPacks; ++k) T::unpack(next[k], v + k * kVec);
     if (tile + 1 < tiles) {
 #pragma unroll
-      for (int k = 0; k < kPacks; ++k) next[k] = loadPack<T, false>(x, place(tile + 1, k, threadIdx.x), end, kNothing);
+      for (int k = 0; k < kPacks; ++k) next[k] = loadPack<T>(x, place(tile + 1, k, threadIdx.x), end, kNothing);
     }
     float most = v[0];
 #pragma unroll
@@ -272,41 +337,52 @@ __global__ __launch_bounds__(kBlock) void logprobKernel(ForwardArgs a) {
       shift = wide ? 0.0f : -to * c;
       rest = wide ? 0.0f : __builtin_fmaf(-to, c, -shift);
     }
-    float t1 = 0.0f;
+    // (the empty asm statements keep the three loops apart: with what they have in common
+    // merged in front of or behind the branches, all of a tile's exponentials would sit in
+    // registers at once: 156 registers and three waves per SIMD instead of 80 and six)
+    float t0 = 0.0f, t1 = 0.0f;
     if (wide) {
 #pragma unroll
       for (int i = 0; i < kLane; ++i) {
         const float y = (v[i] - reference) * c, e = __builtin_amdgcn_exp2f(y);
-        s0 += e;
+        t0 += e;
         if constexpr (kEntropy) t1 = __builtin_fmaf(e, fmaxf(y, -160.0f), t1);
       }
+      asm volatile("" : "+v"(t0), "+v"(t1));
     } else if (kEntropy && masked) {
+      float factor = c;
+      asm volatile("" : "+v"(factor));
 #pragma unroll
       for (int i = 0; i < kLane; ++i) {
-        const float y = __builtin_fmaf(v[i], c, shift), e = __builtin_amdgcn_exp2f(y);
-        s0 += e;
+        const float y = __builtin_fmaf(v[i], factor, shift), e = __builtin_amdgcn_exp2f(y);
+        t0 += e;
         t1 = __builtin_fmaf(e, fmaxf(y, -160.0f), t1);
       }
+      asm volatile("" : "+v"(t0), "+v"(t1));
     } else {
 #pragma unroll
       for (int i = 0; i < kLane; ++i) {
         const float y = __builtin_fmaf(v[i], c, shift), e = __builtin_amdgcn_exp2f(y); // 0 below 2^-149, NaN for NaN
-        s0 += e;
+        t0 += e;
         if constexpr (kEntropy) t1 = __builtin_fmaf(e, y, t1);
       }
+      asm volatile("" : "+v"(t0), "+v"(t1));
       if constexpr (kEntropy) {
         // 0 * -infinity is no term: from the first one on the wave clamps its exponents
         masked = __any(t1 != t1);
         if (masked) {
           t1 = 0.0f;
+          float again = c; // opaque: this loop happens once per wave and is not to be merged into the one above
+          asm volatile("" : "+v"(again));
 #pragma unroll
           for (int i = 0; i < kLane; ++i) {
-            const float y = __builtin_fmaf(v[i], c, shift);
+                const float y = __builtin_fmaf(v[i], again, shift);
             t1 = __builtin_fmaf(__builtin_amdgcn_exp2f(y), fmaxf(y, -160.0f), t1);
           }
         }
       }
     }
+    s0 += t0;
     if constexpr (kEntropy) s1 += t1;
   }
 
@@ -322,8 +398,9 @@ __global__ __launch_bounds__(kBlock) void logprobKernel(ForwardArgs a) {
     uint64_t* keys = reinterpret_cast<uint64_t*>(area);
     const bool some = place(0, 0, threadIdx.x) < end;
     if (threadIdx.x == 0) listed = found = 0;
-    const uint32_t least = laneBound(some ? orderOf(laneBest) : 0u, a.top, scratch);
+    const uint32_t least = laneBound<T::kOrderBits>(some ? orderOf(laneBest) : 0u, a.top, scratch);
     auto listSegments = [&](uint32_t from) { // those whose maximum's order is not below `from`
+#pragma unroll 4
       for (uint32_t tile = 0; tile < tiles; ++tile) {
         const uint32_t order = orderOf(segments[tile * kBlock + threadIdx.x]);
         if (order >= from && order != 0) {
@@ -332,12 +409,53 @@ __global__ __launch_bounds__(kBlock) void logprobKernel(ForwardArgs a) {
         }
       }
     };
-    if (orderOf(laneBest) >= least) listSegments(least);
+    // Few segments: their packs are looked at, one by each lane.  A part of one tile has them in registers
+    // still and puts them into LDS (behind the keys) instead of loading them again.
+    Pack* staged = reinterpret_cast<Pack*>(area + kStagedAt);
+    if (orderOf(laneBest) >= least) {
+      if (tiles > 1) {
+        listSegments(least);
+      } else if (some) {
+        const uint32_t at = atomicAdd(&listed, 1u);
+        if (at < kShortList) {
+          list[at] = static_cast<uint16_t>(threadIdx.x);
+#pragma unroll
+          for (int k = 0; k < kPacks; ++k) staged[at * kPacks + k] = next[k];
+        }
+      }
+    }
     __syncthreads();
-    uint64_t bound = uint64_t(least) << 32; // of the logits' keys
-    const uint16_t* looked = list;
-    uint32_t count = listed;
-    if (count > kShortList) { // uniform
+    bool exact = listed > kShortList; // uniform: too many reach the bound
+    if (!exact) {
+      const uint32_t lowest = orderOf(-__builtin_inff());
+      const float low = least <= lowest ? -__builtin_inff() : valueOf(least); // orders below -infinity's are no numbers
+      const uint32_t room = tiles > 1 ? kMaxListed : kStagedAt / sizeof(uint64_t), packs = listed * kPacks;
+      for (uint32_t e = threadIdx.x; e < packs; e += kBlock) {
+        const uint32_t segment = list[e / kPacks];
+        const uint32_t from = place(segment / kBlock, e % kPacks, segment % kBlock);
+        float w[kVec];
+        T::unpack(tiles > 1 ? loadPack<T, false>(x, from, end, kNothing) : staged[e], w);
+        uint32_t n = 0;
+#pragma unroll
+        for (int i = 0; i < kVec; ++i) n += w[i] >= low && from + i < end;
+        if (n == 0) continue;
+        uint32_t at = atomicAdd(&found, n);
+#pragma unroll
+        for (int i = 0; i < kVec; ++i)
+          if (w[i] >= low && from + i < end) {
+            if (at < room) keys[at] = keyOf(w[i], from + i);
+            ++at;
+          }
+      }
+      __syncthreads();
+      exact = found > room;
+      if (exact) { // of one tile; the keys lie where the maxima were
+        __syncthreads();
+        segments[threadIdx.x] = some ? laneBest : __builtin_nanf("");
+      }
+    }
+    if (exact) {
+      const uint16_t* looked = list;
       // first place of a segment's maximum
       auto segmentKey = [&](uint32_t tile, uint32_t lane, float most) {
         uint32_t at = 0xffffffffu;
@@ -369,15 +487,15 @@ __global__ __launch_bounds__(kBlock) void logprobKernel(ForwardArgs a) {
       const uint64_t bound1 = __shfl(sorted, a.top - 1, 64);
       if (lane == 0) waveBound[threadIdx.x / 64] = bound1;
       __syncthreads(); // everyone has read the first list's length
-      if (threadIdx.x == 0) listed = 0;
+      if (threadIdx.x == 0) listed = found = 0;
       __syncthreads();
-      bound = waveBound[0];
+      uint64_t bound = waveBound[0];
 #pragma unroll
       for (int w = 1; w < kWaves; ++w) bound = bound > waveBound[w] ? bound : waveBound[w];
       // of at most k lanes per wave the segments that may reach the bound: at most kMaxListed
       if (laneKey != 0 && laneKey >= bound) listSegments(static_cast<uint32_t>(bound >> 32));
       __syncthreads(); // the list is whole, and the maxima are not needed any more
-      count = listed;
+      uint32_t count = listed;
       if (count > a.top) {
         for (uint32_t e = threadIdx.x; e < count; e += kBlock) {
           const uint32_t tile = list[e] / kBlock, owner = list[e] % kBlock;
@@ -403,16 +521,16 @@ __global__ __launch_bounds__(kBlock) void logprobKernel(ForwardArgs a) {
         count = a.top;
         looked = kept;
       }
-    }
-    for (uint32_t e = threadIdx.x; e < count * kPacks; e += kBlock) {
-      const uint32_t segment = looked[e / kPacks];
-      const uint32_t from = place(segment / kBlock, e % kPacks, segment % kBlock);
-      float w[kVec];
-      T::unpack(loadPack<T, false>(x, from, end, kNothing), w);
+      for (uint32_t e = threadIdx.x; e < count * kPacks; e += kBlock) {
+        const uint32_t segment = looked[e / kPacks];
+        const uint32_t from = place(segment / kBlock, e % kPacks, segment % kBlock);
+        float w[kVec];
+        T::unpack(loadPack<T, false>(x, from, end, kNothing), w);
 #pragma unroll
-      for (int i = 0; i < kVec; ++i)
-        if (from + i < end && w[i] == w[i] && keyOf(w[i], from + i) >= bound)
-          keys[atomicAdd(&found, 1u)] = keyOf(w[i], from + i);
+        for (int i = 0; i < kVec; ++i)
+          if (from + i < end && w[i] == w[i] && keyOf(w[i], from + i) >= bound)
+            keys[atomicAdd(&found, 1u)] = keyOf(w[i], from + i);
+      }
     }
     __syncthreads();
     if (threadIdx.x < kMaxTop) best[threadIdx.x] = 0;
@@ -423,74 +541,25 @@ __global__ __launch_bounds__(kBlock) void logprobKernel(ForwardArgs a) {
   RowSums total = waveSums[0];
 #pragma unroll
   for (int w = 1; w < kWaves; ++w) total = join(total, waveSums[w], c);
-  if (a.parts == 1) {
-    finishRow(a, row, given, total, best);
-  } else {
-    const uint64_t slot = uint64_t(blockIdx.x);
-    if (threadIdx.x == 0) a.partSums[slot] = total;
-    if (kTop && threadIdx.x < a.top) a.partKeys[slot * a.top + threadIdx.x] = best[threadIdx.x];
-  }
-}
-
-// Joins the parts of a row: one work-group per row.  The sums: a lane per part,
-// in the first wave.  The keys: those that reach the bound that the lanes' best
-// ones give, ranked; where they are too many (logits that are equal all over
-// the row), stretches of the keys are ranked together with the best so far.
-constexpr uint32_t kJoinKeys = 2048;
-template <typename T>
-__global__ __launch_bounds__(kBlock) void logprobJoinKernel(ForwardArgs a) {
-  __shared__ uint64_t keys[kJoinKeys];
-  __shared__ uint64_t best[kMaxTop];
-  __shared__ BoundScratch scratch;
-  __shared__ RowSums sums;
-  __shared__ uint32_t listed;
-  const uint64_t row = a.firstRow + blockIdx.x, slot = uint64_t(blockIdx.x) * a.parts;
-  const float c = a.scale * kLog2e;
-  const Given given = givenOf<T>(a, row);
-  if (threadIdx.x < 64) {
-    RowSums r{-__builtin_inff(), 0.0f, 0.0f};
-    for (uint32_t p = threadIdx.x; p < a.parts; p += 64) r = join(r, a.partSums[slot + p], c);
-    const float m = waveMax(r.m);
-    const float d = rebase(r.m, m, c), f = __builtin_amdgcn_exp2f(d);
-    const float s1 = waveSum((r.s1 + r.s0 * d) * f), s0 = waveSum(r.s0 * f);
-    if (threadIdx.x == 0) sums = RowSums{m, s0, s1};
-  }
-  if (a.top != 0) {
-    const uint64_t* from = a.partKeys + slot * a.top;
-    const uint32_t all = a.parts * a.top;
-    uint64_t mine = 0;
-    for (uint32_t e = threadIdx.x; e < all; e += kBlock) mine = from[e] > mine ? from[e] : mine;
-    if (threadIdx.x == 0) listed = 0;
-    const uint32_t least = laneBound(static_cast<uint32_t>(mine >> 32), a.top, scratch);
-    for (uint32_t e = threadIdx.x; e < all; e += kBlock) {
-      const uint64_t key = from[e];
-      if (key != 0 && static_cast<uint32_t>(key >> 32) >= least) {
-        const uint32_t at = atomicAdd(&listed, 1u);
-        if (at < kJoinKeys) keys[at] = key;
-      }
+  if (a.parts > 1) {
+    const uint32_t rowInLaunch = blockIdx.x / a.parts;
+    if (threadIdx.x < 64) { // all that is written is this wave's, and it waits for it
+      unsigned char* slot = a.slots + uint64_t(blockIdx.x) * a.slotBytes;
+      if (threadIdx.x == 0) putPart(slot, total.m), putPart(slot + 4, total.s0), putPart(slot + 8, total.s1);
+      if (kTop && threadIdx.x < a.top) putPart(slot + kSumsBytes + threadIdx.x * sizeof(uint64_t), best[threadIdx.x]);
+      asm volatile("s_waitcnt vmcnt(0)" ::: "memory");
+      if (threadIdx.x == 0)
+        listed = __hip_atomic_fetch_add(&a.arrived[rowInLaunch], 1u, __ATOMIC_RELAXED, __HIP_MEMORY_SCOPE_AGENT) + 1 == a.parts;
     }
-    if (threadIdx.x < kMaxTop) best[threadIdx.x] = 0;
     __syncthreads();
-    if (listed <= kJoinKeys) { // uniform
-      rankKeys(keys, listed, a.top, [&](uint32_t rank, uint64_t key, uint32_t) { best[rank] = key; });
-    } else {
-      for (uint32_t at = 0; at < all; at += kJoinKeys - kMaxTop) {
-        const uint32_t count = all - at < kJoinKeys - kMaxTop ? all - at : kJoinKeys - kMaxTop;
-        __syncthreads();
-        for (uint32_t e = threadIdx.x; e < count; e += kBlock) keys[e] = from[at + e];
-        if (threadIdx.x < a.top) keys[count + threadIdx.x] = best[threadIdx.x];
-        __syncthreads();
-        if (threadIdx.x < kMaxTop) best[threadIdx.x] = 0;
-        __syncthreads();
-        // empty places (key 0) are not distinct, but rank below every logit
-        rankKeys(keys, count + a.top, a.top, [&](uint32_t rank, uint64_t key, uint32_t) {
-          if (key != 0) best[rank] = key;
-        });
-      }
-    }
+    if (listed == 0) return; // the whole work-group
+    if (threadIdx.x == 0) __hip_atomic_store(&a.arrived[rowInLaunch], 0u, __ATOMIC_RELAXED, __HIP_MEMORY_SCOPE_AGENT);
+    const unsigned char* slots = a.slots + uint64_t(rowInLaunch) * a.parts * a.slotBytes;
+    total = joinSums(slots, a.slotBytes, a.parts, c);
+    if constexpr (kTop)
+      joinKeys<T>(slots, a.slotBytes, a.parts, a.top, reinterpret_cast<uint64_t*>(area), best, scratch, &found);
   }
-  __syncthreads();
-  finishRow(a, row, given, sums, best);
+  finishRow(a, row, given, total, best);
 }
 
 // ---- gradient ----------------------------------------------------------------------
@@ -561,23 +630,23 @@ template <typename T> int forward(polar_hip_device* dev, ForwardArgs a, uint64_t
   const bool entropy = a.entropy != nullptr, top = a.top != 0;
   auto kernel = entropy ? (top ? logprobKernel<T, true, true> : logprobKernel<T, true, false>)
                         : (top ? logprobKernel<T, false, true> : logprobKernel<T, false, false>);
-  // rows per launch: block numbers in 31 bits, parts' results in 64 MiB of workspace
-  const uint64_t slotBytes = sizeof(RowSums) + uint64_t(a.top) * sizeof(uint64_t);
+  // rows per launch: work-group numbers in 31 bits, parts' slots in 64 MiB of workspace, a counter per row
+  a.slotBytes = static_cast<uint32_t>((kSumsBytes + a.top * sizeof(uint64_t) + 127) / 128 * 128);
   uint64_t batch = (1ull << 30) / a.parts;
-  if (a.parts > 1) batch = std::min(batch, std::max<uint64_t>(1, (64ull << 20) / (a.parts * slotBytes)));
+  if (a.parts > 1)
+    batch = std::min({batch, uint64_t(kTileCounters), std::max<uint64_t>(1, (64ull << 20) / (uint64_t(a.parts) * a.slotBytes))});
   std::lock_guard<std::mutex> lock(dev->workspaceMu);
   for (uint64_t r = 0; r < rows; r += batch) {
     const uint64_t n = std::min(batch, rows - r);
     a.firstRow = r;
     if (a.parts > 1) {
       void* area = nullptr;
-      const int st = workspaceFor(dev, n * a.parts * slotBytes, &area);
+      const int st = workspaceFor(dev, n * a.parts * a.slotBytes, &area);
       if (st != POLAR_HIP_OK) return st;
-      a.partKeys = static_cast<uint64_t*>(area);
-      a.partSums = reinterpret_cast<RowSums*>(a.partKeys + n * a.parts * a.top);
+      a.slots = static_cast<unsigned char*>(area);
+      a.arrived = dev->tileCounters;
     }
     POLAR_HIP_TRY(launchKernel(dev, kernel, dim3(static_cast<unsigned>(n * a.parts)), dim3(kBlock), a));
-    if (a.parts > 1) POLAR_HIP_TRY(launchKernel(dev, logprobJoinKernel<T>, dim3(static_cast<unsigned>(n)), dim3(kBlock), a));
   }
   return POLAR_HIP_OK;
 }

@@ -21,6 +21,7 @@ typedef _Float16 F16x2 __attribute__((ext_vector_type(2)));
 struct TypeF32 {
   using Stored = float;
   static constexpr int kVec = 4; // elements in a Pack
+  static constexpr int kOrderBits = 20; // leading bits of an fp32 that tell values apart well enough to bound them
   using At = PackAt4;
   __device__ static float widen(float v) { return v; }
   __device__ static float narrow(float v) { return v; }
@@ -42,6 +43,7 @@ struct TypeF32 {
 struct TypeF16 {
   using Stored = _Float16;
   static constexpr int kVec = 8;
+  static constexpr int kOrderBits = 20; // sign, eight bits of exponent, ten of mantissa: all there is
   using At = PackAt2;
   __device__ static float widen(_Float16 v) { return static_cast<float>(v); }
   __device__ static _Float16 narrow(float v) { return static_cast<_Float16>(v); } // to nearest, ties to even
@@ -66,6 +68,7 @@ struct TypeF16 {
 struct TypeBF16 {
   using Stored = __bf16;
   static constexpr int kVec = 8;
+  static constexpr int kOrderBits = 16; // all there is
   using At = PackAt2;
   __device__ static float widen(__bf16 v) { return static_cast<float>(v); }
   __device__ static __bf16 narrow(float v) { return static_cast<__bf16>(v); } // to nearest, ties to even
