@@ -404,7 +404,7 @@ typedef struct polar_hip_adamw_tensor {
                       /* fp32, of which param gets a rounded copy                  */
   float* m_scale;     /* 8-bit states: one per 256 elements; else not used         */
   float* v_scale;
-  uint64_t count;     /* may be 0: the tensor is passed over                      */
+  uint64_t count;     /* up to 2^33; 0: the tensor is passed over                 */
   uint64_t first;     /* number of the tensor's first element in the sequence of   */
                       /* random numbers: the elements of the tensors before it     */
   double weight_decay;
@@ -424,7 +424,9 @@ typedef struct polar_hip_adamw_config {
  * The list is read before the call returns.  All of it is checked before
  * anything is launched.  Tensors must not overlap.  8-bit states are rounded
  * stochastically, up where the upper (v) or lower (m) 16 bits of a hash of seed
- * and element number say so; a block whose scale is below 2^-100 holds zeros. */
+ * and element number say so; a block whose scale is not above 2^-100 holds zeros,
+ * and a state that is not finite is held as NaN, without a say in its block's
+ * scale. */
 int polar_hip_fadamw(polar_hip_device* dev, const polar_hip_adamw_config* config,
                      const polar_hip_adamw_tensor* tensors, uint64_t count);
 

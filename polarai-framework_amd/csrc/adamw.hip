@@ -3,11 +3,15 @@
 //   g = gradScale * grad,  m = b1 m + (1 - b1) g,  v = b2 v + (1 - b2) g^2
 //   p = p - lr wd p - (lr / (1 - b1^t)) m / (sqrt(v) / sqrt(1 - b2^t) + eps)
 //
-// Everything is read once and written once.  A launch covers up to kTensors
-// tensors, whose table travels in the kernel's arguments: no table in device
-// memory to upload and keep, and a model of a few hundred tensors takes a few
-// launches.  A work-group takes a chunk of kChunk elements of one tensor; a
-// lane takes four consecutive elements at a time.
+// Everything is read once and written once: memory is what bounds it.  100
+// million elements in fp32 (28 bytes each) take 457 us, 6.2 TB/s, 91 % of what
+// a large copy reaches; 260 million with states in 8 bits, bf16 gradients and
+// copies (16 bytes each) 708 us, 6.1 TB/s.  Loads and stores stream past the
+// caches (with plain loads or plain stores 510 us).  A launch covers up to
+// kTensors tensors, whose table travels in the kernel's arguments: no table in
+// device memory to upload and keep, and a model of a few hundred tensors takes
+// a few launches.  A work-group takes a chunk of one tensor, a lane four
+// consecutive elements of it.
 //
 // States in 8 bits: 256 consecutive elements of a tensor (one wave's four per
 // lane) share a scale, the largest value in the block / 448.  m is held as an
@@ -28,15 +32,18 @@ using namespace polar_hip_detail;
 
 namespace {
 
-constexpr int kBlock = 256;
-constexpr int kRounds = 4;                          // groups of four elements per lane
-constexpr uint32_t kChunk = kBlock * 4 * kRounds;   // elements of a work-group
+// Small work-groups with one group of four elements per lane measured best, as for the
+// elementwise kernels: 100 million fp32 elements 457 us, with 256 lanes 500, with two or four
+// groups per lane 490
+constexpr int kBlock = 128;
+constexpr uint32_t kChunk = kBlock * 4;             // elements of a work-group
 constexpr uint64_t kScaleBlock = POLAR_HIP_ADAMW_BLOCK; // elements that share a scale
 static_assert(kScaleBlock == 64 * 4, "one wave's four elements per lane");
 constexpr float kLargest = 448.0f;                  // of the 8-bit floats
 constexpr float kTiny = 0x1p-100f;                  // blocks whose scale is not above this are held as zeros
 
-constexpr int kTensors = 40;
+constexpr uint64_t kMostGroups = 1ull << 24; // of a launch, whose lanes are counted in 32 bits
+constexpr int kTensors = 46;
 struct Entry {
   void *param, *grad, *m, *v;
   float *master, *mScale, *vScale;
@@ -55,7 +62,7 @@ template <int kBytes> struct Words;
 template <> struct Words<16> { typedef uint32_t At __attribute__((ext_vector_type(4), aligned(4))); };
 template <> struct Words<8> { typedef uint32_t At __attribute__((ext_vector_type(2), aligned(2))); };
 
-// four consecutive elements, the first `n` of them real (1 .. 4)
+// four consecutive elements, the first `n` of them real (0 .. 4)
 template <typename T>
 __device__ __forceinline__ void load4(const typename T::Stored* at, int n, float* out) {
   using S = typename T::Stored;
@@ -109,16 +116,32 @@ __device__ __forceinline__ void widenCodes(uint32_t w, float* out) {
   const Float2 low = __builtin_amdgcn_cvt_pk_f32_fp8(w, false), high = __builtin_amdgcn_cvt_pk_f32_fp8(w, true);
   out[0] = low.x, out[1] = low.y, out[2] = high.x, out[3] = high.y;
 }
-// |t| <= 448 as an 8-bit float, up where 16 random bits exceed what is cut off:
-// among the normal ones by adding them below the mantissa's last kept bit (the
-// carry may reach the exponent, which is the next float), below 2^-6 in steps of
-// 2^-9
+// A value of at most 448 (and a rounding error) in size as an 8-bit float, up where 16
+// random bits exceed what is cut off: among the normal ones by adding them below the
+// mantissa's last kept bit (the carry may reach the exponent, which is the next float),
+// below 2^-6 in steps of 2^-9
 __device__ __forceinline__ uint32_t narrowCode(float t, uint32_t random) {
+  const uint32_t bits = __builtin_bit_cast(uint32_t, t);
   const float size = fabsf(t);
-  const uint32_t normal = ((__builtin_bit_cast(uint32_t, size) + (random << 4)) >> 20) - (120u << 3);
+  const uint32_t normal = (((bits & 0x7fffffffu) + (random << 4)) >> 20) - (120u << 3);
   const uint32_t small = static_cast<uint32_t>(size * 512.0f + static_cast<float>(random) * (1.0f / 65536.0f));
   const uint32_t code = size >= 0x1p-6f ? (normal < 0x7eu ? normal : 0x7eu) : small;
-  return code | (t < 0.0f ? 0x80u : 0u);
+  return code | ((bits >> 24) & 0x80u);
+}
+constexpr uint32_t kNotANumber = 0x7f; // as an 8-bit float
+constexpr uint32_t kInfinity = 0x7f800000u;
+
+// Largest of the wave's sizes, given as the bits of fp32 numbers that are not negative:
+// in their order, NaN above infinity
+__device__ __forceinline__ uint32_t waveLargest(uint32_t v) {
+  auto step = [](uint32_t x, auto move) { return max(x, static_cast<uint32_t>(move(static_cast<int>(x)))); };
+  v = step(v, [](int x) { return __builtin_amdgcn_update_dpp(x, x, 0xb1, 0xf, 0xf, false); });
+  v = step(v, [](int x) { return __builtin_amdgcn_update_dpp(x, x, 0x4e, 0xf, 0xf, false); });
+  v = step(v, [](int x) { return __builtin_amdgcn_update_dpp(x, x, 0x141, 0xf, 0xf, false); });
+  v = step(v, [](int x) { return __builtin_amdgcn_update_dpp(x, x, 0x140, 0xf, 0xf, false); });
+  v = step(v, [](int x) { return __builtin_amdgcn_update_dpp(x, x, 0x142, 0xa, 0xf, false); });
+  v = step(v, [](int x) { return __builtin_amdgcn_update_dpp(x, x, 0x143, 0xc, 0xf, false); });
+  return static_cast<uint32_t>(__builtin_amdgcn_readlane(static_cast<int>(v), 63));
 }
 
 // 32 random bits of an element: a multiply-xorshift hash of its number and the
@@ -131,34 +154,19 @@ __device__ __forceinline__ uint32_t randomBits(uint32_t seed, uint64_t element) 
   return h ^ (h >> 16);
 }
 
-// P: the parameter's type; one of 16 bits is a copy of the fp32 master.  G: the gradient's.
-template <typename P, typename G, bool kSmall>
-__global__ __launch_bounds__(kBlock) void adamwKernel(Table table) {
-  constexpr bool kCopy = sizeof(typename P::Stored) == 2;
-  // all the first groups sit side by side in scalar registers: no search through memory
-  int which = 0;
-  uint32_t first = 0;
-#pragma unroll
-  for (int i = 1; i < kTensors; ++i) {
-    const bool behind = blockIdx.x >= table.firstGroup[i];
-    which += behind;
-    first = behind ? table.firstGroup[i] : first;
-  }
-  const Entry e = table.e[which];
-  const uint64_t base = uint64_t(blockIdx.x - first) * kChunk + threadIdx.x * 4;
-  float* master = kCopy ? e.master : static_cast<float*>(e.param);
-#pragma unroll
-  for (int round = 0; round < kRounds; ++round) {
-    const uint64_t at = base + uint64_t(round) * kBlock * 4;
-    const int n = at >= e.count ? 0 : e.count - at < 4 ? static_cast<int>(e.count - at) : 4;
-    // a wave whose block of 256 lies behind the tensor's end has nothing to do
-    if (kSmall ? at - threadIdx.x % 64 * 4 >= e.count : n == 0) break;
-    float p[4], g[4], m[4], v[4], r[4];
-    const uint64_t block = at / kScaleBlock;
+// Four consecutive elements of a tensor in a lane, `n` of them (0 .. 4) real.  P: the
+// parameter's type; one of 16 bits is a copy of the fp32 master.  G: the gradient's.
+template <typename P, typename G, bool kSmall> struct Four {
+  float p[4], g[4], m[4], v[4], r[4];
+
+  __device__ __forceinline__ void load(const Entry& e, const float* master, uint64_t at, int n) {
+    load4<TypeF32>(master + at, n, p);
+    load4<G>(static_cast<const typename G::Stored*>(e.grad) + at, n, g);
     if constexpr (kSmall) {
+      const uint64_t block = at / kScaleBlock;
       const float ms = e.mScale[block], vs = e.vScale[block];
-      widenCodes(n ? loadCodes(static_cast<const uint8_t*>(e.m) + at, n) : 0u, m);
-      widenCodes(n ? loadCodes(static_cast<const uint8_t*>(e.v) + at, n) : 0u, r);
+      widenCodes(loadCodes(static_cast<const uint8_t*>(e.m) + at, n), m);
+      widenCodes(loadCodes(static_cast<const uint8_t*>(e.v) + at, n), r);
 #pragma unroll
       for (int i = 0; i < 4; ++i) {
         m[i] *= ms;
@@ -169,49 +177,106 @@ __global__ __launch_bounds__(kBlock) void adamwKernel(Table table) {
       load4<TypeF32>(static_cast<const float*>(e.m) + at, n, m);
       load4<TypeF32>(static_cast<const float*>(e.v) + at, n, v);
     }
-    load4<TypeF32>(master + at, n, p);
-    load4<G>(static_cast<const typename G::Stored*>(e.grad) + at, n, g);
+  }
+
+  __device__ __forceinline__ void step(const Table& t, float decay) {
 #pragma unroll
     for (int i = 0; i < 4; ++i) {
-      g[i] *= table.gradScale;
-      m[i] = m[i] * table.beta1 + g[i] * table.rest1;
-      v[i] = v[i] * table.beta2 + (g[i] * g[i]) * table.rest2;
-      r[i] = sqrtf(v[i]);
-      p[i] = (p[i] - p[i] * e.decay) - (m[i] * table.stepSize) / (r[i] * table.byCorrection + table.eps);
+      g[i] *= t.gradScale;
+      m[i] = m[i] * t.beta1 + g[i] * t.rest1;
+      v[i] = v[i] * t.beta2 + (g[i] * g[i]) * t.rest2;
+      const float scaled = m[i] * t.stepSize;
+      if constexpr (kSmall) {
+        // the hardware's square root and reciprocal, each good to a unit in the last place: against states
+        // of three bits and a parameter that the quotient changes by a thousandth that is nothing, and the
+        // exact sequences' 20 instructions per element would set the time (788 us for 260 million elements
+        // instead of 708).  The divisor is 0, or far above the subnormal numbers: a root's smallest value
+        // is 3.7e-23.
+        r[i] = __builtin_amdgcn_sqrtf(v[i]);
+        p[i] = (p[i] - p[i] * decay) - scaled * __builtin_amdgcn_rcpf(r[i] * t.byCorrection + t.eps);
+      } else {
+        r[i] = sqrtf(v[i]);
+        p[i] = (p[i] - p[i] * decay) - scaled / (r[i] * t.byCorrection + t.eps);
+      }
     }
-    if (n) {
-      store4<TypeF32>(master + at, n, p);
-      if constexpr (kCopy) store4<P>(static_cast<typename P::Stored*>(e.param) + at, n, p);
-    }
+  }
+
+  __device__ __forceinline__ void store(const Table& t, const Entry& e, float* master, uint64_t at, int n) {
+    store4<TypeF32>(master + at, n, p);
+    if constexpr (sizeof(typename P::Stored) == 2) store4<P>(static_cast<typename P::Stored*>(e.param) + at, n, p);
     if constexpr (kSmall) {
       // elements behind the end are zeros: loads give them as such, and they stay
-      float largestM = 0.0f, largestR = 0.0f;
+      uint32_t largestM = 0, largestR = 0;
 #pragma unroll
       for (int i = 0; i < 4; ++i) {
-        largestM = fmaxf(largestM, fabsf(m[i]));
-        largestR = fmaxf(largestR, r[i]);
+        largestM = max(largestM, __builtin_bit_cast(uint32_t, fabsf(m[i])));
+        largestR = max(largestR, __builtin_bit_cast(uint32_t, fabsf(r[i])));
       }
-      const float ms = waveMax(largestM) * (1.0f / kLargest), vs = waveMax(largestR) * (1.0f / kLargest);
+      largestM = waveLargest(largestM), largestR = waveLargest(largestR);
+      const bool odd = largestM >= kInfinity || largestR >= kInfinity; // rare, and the whole wave's
+      if (odd) {
+        // an element that is not finite is held as NaN and has no say in its block's scale
+        largestM = largestR = 0;
+#pragma unroll
+        for (int i = 0; i < 4; ++i) {
+          const uint32_t bitsM = __builtin_bit_cast(uint32_t, fabsf(m[i])), bitsR = __builtin_bit_cast(uint32_t, fabsf(r[i]));
+          largestM = max(largestM, bitsM < kInfinity ? bitsM : 0u);
+          largestR = max(largestR, bitsR < kInfinity ? bitsR : 0u);
+        }
+        largestM = waveLargest(largestM), largestR = waveLargest(largestR);
+      }
+      const float ms = __builtin_bit_cast(float, largestM) * (1.0f / kLargest);
+      const float vs = __builtin_bit_cast(float, largestR) * (1.0f / kLargest);
       const float byM = ms > kTiny ? 1.0f / ms : 0.0f, byV = vs > kTiny ? 1.0f / vs : 0.0f;
       uint32_t codeM = 0, codeV = 0;
 #pragma unroll
       for (int i = 0; i < 4; ++i) {
-        const uint32_t random = randomBits(table.seed, e.random + at + i);
-        codeM |= narrowCode(fminf(fmaxf(m[i] * byM, -kLargest), kLargest), random & 0xffffu) << (8 * i);
-        codeV |= narrowCode(fminf(r[i] * byV, kLargest), random >> 16) << (8 * i);
+        const uint32_t random = randomBits(t.seed, e.random + at + i);
+        codeM |= narrowCode(m[i] * byM, random & 0xffffu) << (8 * i);
+        codeV |= narrowCode(r[i] * byV, random >> 16) << (8 * i);
       }
-      if (n) {
-        storeCodes(static_cast<uint8_t*>(e.m) + at, n, codeM);
-        storeCodes(static_cast<uint8_t*>(e.v) + at, n, codeV);
+      if (odd) {
+#pragma unroll
+        for (int i = 0; i < 4; ++i) {
+          if (!(fabsf(m[i]) < __builtin_inff())) codeM = (codeM & ~(0xffu << (8 * i))) | kNotANumber << (8 * i);
+          if (!(fabsf(r[i]) < __builtin_inff())) codeV = (codeV & ~(0xffu << (8 * i))) | kNotANumber << (8 * i);
+        }
       }
+      storeCodes(static_cast<uint8_t*>(e.m) + at, n, codeM);
+      storeCodes(static_cast<uint8_t*>(e.v) + at, n, codeV);
       if (threadIdx.x % 64 == 0) {
-        e.mScale[block] = ms;
-        e.vScale[block] = vs;
+        e.mScale[at / kScaleBlock] = ms;
+        e.vScale[at / kScaleBlock] = vs;
       }
     } else {
       store4<TypeF32>(static_cast<float*>(e.m) + at, n, m);
       store4<TypeF32>(static_cast<float*>(e.v) + at, n, v);
     }
+  }
+};
+
+template <typename P, typename G, bool kSmall>
+__global__ __launch_bounds__(kBlock) void adamwKernel(Table table) {
+  constexpr bool kCopy = sizeof(typename P::Stored) == 2;
+  // all the first groups sit side by side in scalar registers: no search through memory
+  int which = 0;
+#pragma unroll
+  for (int i = 1; i < kTensors; ++i) which = blockIdx.x >= table.firstGroup[i] ? i : which;
+  which = __builtin_amdgcn_readfirstlane(which);
+  const uint32_t first = table.firstGroup[which];
+  const Entry e = table.e[which];
+  const uint64_t at = uint64_t(blockIdx.x - first) * kChunk + threadIdx.x * 4;
+  float* master = kCopy ? e.master : static_cast<float*>(e.param);
+  Four<P, G, kSmall> f;
+  if (at - threadIdx.x * 4 + kChunk <= e.count) { // a whole chunk: no element is checked
+    f.load(e, master, at, 4);
+    f.step(table, e.decay);
+    f.store(table, e, master, at, 4);
+  } else if (at - threadIdx.x % 64 * 4 < e.count) { // not a wave that lies behind the tensor's end as a whole
+    const int n = at >= e.count ? 0 : e.count - at < 4 ? static_cast<int>(e.count - at) : 4;
+    f.load(e, master, at, n);
+    f.step(table, e.decay);
+    f.store(table, e, master, at, n);
   }
 }
 
@@ -247,7 +312,7 @@ int polar_hip_fadamw(polar_hip_device* dev, const polar_hip_adamw_config* config
     const polar_hip_adamw_tensor& t = tensors[i];
     POLAR_HIP_REQUIRE(std::isfinite(t.weight_decay), "a tensor's weight decay is not finite");
     if (t.count == 0) continue;
-    POLAR_HIP_REQUIRE(t.count < (1ull << 42), "a tensor is too large");
+    POLAR_HIP_REQUIRE(t.count <= kChunk * kMostGroups, "a tensor is too large");
     POLAR_HIP_REQUIRE(t.param && t.grad && t.m && t.v, "a tensor's pointer is null");
     POLAR_HIP_REQUIRE(!copy || t.master, "16-bit parameters need an fp32 master");
     POLAR_HIP_REQUIRE(!small || (t.m_scale && t.v_scale), "8-bit states need scales");
@@ -272,7 +337,6 @@ int polar_hip_fadamw(polar_hip_device* dev, const polar_hip_adamw_config* config
   const Kernel kernel = config->param_type == POLAR_HIP_F32   ? pick<TypeF32>(config->grad_type, small)
                         : config->param_type == POLAR_HIP_F16 ? pick<TypeF16>(config->grad_type, small)
                                                               : pick<TypeBF16>(config->grad_type, small);
-  constexpr uint64_t kMostGroups = 1ull << 30; // of a launch
   uint64_t groups = 0;
   int listed = 0;
   auto flush = [&]() -> int {
@@ -286,7 +350,7 @@ int polar_hip_fadamw(polar_hip_device* dev, const polar_hip_adamw_config* config
   for (uint64_t i = 0; i < count; ++i) {
     const polar_hip_adamw_tensor& t = tensors[i];
     if (t.count == 0) continue;
-    const uint64_t mine = (t.count + kChunk - 1) / kChunk; // below 2^30
+    const uint64_t mine = (t.count + kChunk - 1) / kChunk;
     if (listed == kTensors || groups + mine > kMostGroups) {
       const int st = flush();
       if (st != POLAR_HIP_OK) return st;

@@ -40,6 +40,7 @@ constexpr int kMaxListed = kWaves * kMaxTop * kMaxTiles;  // segments that can r
 constexpr uint32_t kShortList = 64;                       // segments whose logits are looked at without ordering them first
 constexpr uint32_t kStagedAt = 12288;                     // bytes in front of the staged packs of a part of one tile
 constexpr uint64_t kMaxCols = 1ull << 24;                 // places are exact as fp32 tokens
+constexpr uint64_t kMostGroups = 1ull << 23;              // of a launch, whose lanes are counted in 32 bits
 constexpr float kLog2e = 1.44269504088896340736f;
 constexpr float kLn2 = 0.69314718055994530942f;
 
@@ -630,9 +631,9 @@ template <typename T> int forward(polar_hip_device* dev, ForwardArgs a, uint64_t
   const bool entropy = a.entropy != nullptr, top = a.top != 0;
   auto kernel = entropy ? (top ? logprobKernel<T, true, true> : logprobKernel<T, true, false>)
                         : (top ? logprobKernel<T, false, true> : logprobKernel<T, false, false>);
-  // rows per launch: work-group numbers in 31 bits, parts' slots in 64 MiB of workspace, a counter per row
+  // rows per launch: lanes in 32 bits, parts' slots in 64 MiB of workspace, a counter per row
   a.slotBytes = static_cast<uint32_t>((kSumsBytes + a.top * sizeof(uint64_t) + 127) / 128 * 128);
-  uint64_t batch = (1ull << 30) / a.parts;
+  uint64_t batch = kMostGroups / a.parts;
   if (a.parts > 1)
     batch = std::min({batch, uint64_t(kTileCounters), std::max<uint64_t>(1, (64ull << 20) / (uint64_t(a.parts) * a.slotBytes))});
   std::lock_guard<std::mutex> lock(dev->workspaceMu);
@@ -655,7 +656,7 @@ template <typename T> int backward(polar_hip_device* dev, GradArgs a) {
   constexpr uint32_t kChunk = kBlock * kGradPacks * T::kVec;
   a.chunks = (a.cols + kChunk - 1) / kChunk;
   auto kernel = a.dentropy != nullptr ? logprobGradKernel<T, true> : logprobGradKernel<T, false>;
-  const uint64_t batch = (1ull << 30) / a.chunks, rows = a.rows;
+  const uint64_t batch = kMostGroups / a.chunks, rows = a.rows;
   GradArgs part = a;
   for (uint64_t r = 0; r < rows; r += batch) {
     const uint64_t n = std::min(batch, rows - r);

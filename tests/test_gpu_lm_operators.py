@@ -405,6 +405,28 @@ def test_logprob_grad(dev, rows, cols, kind):
         t.free()
 
 
+def test_logprob_of_more_rows_than_a_launch_takes(dev):
+    """One logit per row: log probability and gradient are 0; more work-groups than one launch has."""
+    _say("flogprob 8.5 million rows")
+    rows = (1 << 23) + 12345
+    x = np.random.default_rng(1).standard_normal(rows).astype(np.float32)
+    X, T = Raw(dev, x), Raw(dev, np.zeros(rows, np.int32))
+    LP, S, G = Raw(dev, np.ones(rows, np.float32)), Raw(dev, np.ones((rows, 2), np.float32)), Raw(dev, np.ones(rows, np.float32))
+    TI, TL = Raw(dev, np.full(rows, 9, np.int32)), Raw(dev, np.ones(rows, np.float32))
+    dev.flogprob(X, T, LP, rows, 1, stats=S, top=1, top_index=TI, top_logprob=TL, token_dtype="i32")
+    # the sum is one exponential of (almost) 0 times another: each within a unit in the last place (2 u) of 1, the
+    # product rounds once more, and the logarithm of 1 + 5 u within its own last place: 8 u of 0
+    s = S.values()
+    assert not TI.values().any() and np.array_equal(s[:, 0], x)
+    for v in (LP.values(), TL.values(), s[:, 1]):
+        assert np.abs(v).max() <= 8 * U32
+    dev.flogprob_grad(X, T, S, G, X, rows, 1, token_dtype="i32")
+    # p is e to the power of that, with one more exponential's 2 u: 1 - p is off by 8 u + 2 u and two roundings
+    assert np.abs(X.values()).max() <= 12 * U32
+    for t in (X, T, LP, S, G, TI, TL):
+        t.free()
+
+
 def test_logprob_grad_against_differences_of_the_forward_pass(dev):
     """dlogits of the device against central differences of the 64-bit forward pass."""
     _say("flogprob_grad differences")
@@ -556,6 +578,43 @@ def test_adamw_8_bit_states_follow_on_average(dev):
         assert abs(mean / (want * size) ** 2 - 1) < 0.05, (size, mean, (want * size) ** 2)
     for t in (P, G, M, V, MS, VS):
         t.free()
+
+
+@pytest.mark.parametrize("state", ["f32", "8bit"])
+def test_adamw_keeps_nan_and_infinity_in_their_elements(dev, state):
+    """A gradient that is not finite spoils its own element, now and in the next step, and no other of its block."""
+    _say("fadamw nan", state)
+    rng = np.random.default_rng(14)
+    n = 1000
+    g = rng.standard_normal(n).astype(np.float32) * 0.1
+    bad = np.zeros(n, bool)
+    bad[[7, 300, 999]] = True
+    spoilt = g.copy()
+    spoilt[7], spoilt[300], spoilt[999] = np.nan, np.inf, -np.inf
+    results = []
+    for first in (g, spoilt):
+        P = Raw(dev, np.full(n, 0.5, np.float32))
+        grads = [Raw(dev, first), Raw(dev, g)]
+        code = np.uint8 if state == "8bit" else np.float32
+        M, V = Raw(dev, np.zeros(n, code)), Raw(dev, np.zeros(n, code))
+        MS, VS = Raw(dev, np.zeros(4, np.float32)), Raw(dev, np.zeros(4, np.float32))
+        for step, G in enumerate(grads, 1):
+            dev.fadamw(capi.adamw_tensors([dict(count=n, param=P, grad=G, m=M, v=V, m_scale=MS, v_scale=VS)]), step=step, lr=1e-3,
+                       seed=step, state_dtype=state)
+        results.append((P.values(), MS.values(), VS.values()))
+        for t in (P, M, V, MS, VS, *grads):
+            t.free()
+    (clean, ms, vs), (got, got_ms, got_vs) = results
+    assert not np.isfinite(got[bad]).any() and np.isfinite(got[~bad]).all()
+    if state == "f32":
+        assert np.array_equal(got[~bad], clean[~bad])
+    else:
+        # the scales lack the spoilt elements, no more; a block without one is as it was
+        assert np.isfinite(got_ms).all() and np.isfinite(got_vs).all()
+        assert (got_ms <= ms).all() and np.array_equal(got[512:768], clean[512:768])
+        # an update is lr in size at most about the first steps: sqrt(v) and m of one gradient; the states' rounding
+        # moves it by 1/8 of lr per state
+        assert np.abs(got - clean)[~bad].max() <= 0.25e-3
 
 
 # ---- together ---------------------------------------------------------------------

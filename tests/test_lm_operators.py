@@ -97,7 +97,7 @@ CONFIG = dict(param_type=0, grad_type=0, state_bits=32, seed=1, step=1, lr=1e-3,
     (dict(beta2=float("nan")), {}, "beta1"), (dict(lr=float("inf")), {}, "finite"), (dict(eps=-1.0), {}, "finite"),
     (dict(grad_scale=float("nan")), {}, "finite"), ({}, dict(param=0), "null"), ({}, dict(grad=0), "null"), ({}, dict(m=0), "null"),
     ({}, dict(v=0), "null"), (dict(param_type=2), dict(master=0), "master"), (dict(state_bits=8), dict(m_scale=0), "scales"),
-    (dict(state_bits=8), dict(v_scale=0), "scales"), ({}, dict(count=1 << 42), "too large"),
+    (dict(state_bits=8), dict(v_scale=0), "scales"), ({}, dict(count=(1 << 33) + 1), "too large"),
     ({}, dict(weight_decay=float("nan")), "decay"), ({}, dict(m=A + 1), "misaligned"), ({}, dict(param=A + 2), "misaligned")])
 def test_adamw_refuses(lib, handle, config, tensor, words):
     # the second tensor of the list is the wrong one: nothing is launched for the first either
