@@ -4,17 +4,24 @@
 //   with g = dy w and h = (x - mean) rstd:
 //   dx = rstd (g - mean(g) - h mean(g h)),   dw = sum over rows of dy h,   db = sum over rows of dy
 //
-// A row is held in the registers of 1, 4, 8 or 16 waves (kWaves x 64 lanes x
-// kPacks 16-byte packs), so x and dy are read once from memory although the
+// A row is held in the registers of 1 to 16 waves (kWaves x 64 lanes x kPacks
+// 16-byte packs), so x and dy are read once from memory although the
 // statistics need two passes over them: the variance is the sum of squared
 // distances from the mean already known, never E[x^2] - mean^2, which loses
 // all its digits for rows far from zero.  A team of waves walks over rows
-// team, team + teams, ...: weight and bias stay in its registers, the next row
-// is loaded while the present one is reduced, and in the backward pass the
-// columns' sums for dw and db stay in registers until the team's last row; a
-// second kernel adds the teams' sums in a fixed order (no atomics: the same
-// bits on every run).  Rows that no team's registers hold go through memory
-// (cache) once per pass.
+// team, team + teams, ...: weight and bias stay in its registers, the next
+// kAhead rows are loaded while the present one is reduced, and in the backward
+// pass the columns' sums for dw and db stay in registers until the team's last
+// row; a second kernel adds the teams' sums in a fixed order (no atomics: the
+// same bits on every run).  Rows that no team's registers hold go through
+// memory (cache) once per pass.
+//
+// Memory bounds it.  16384 x 8192 bf16 takes 89 us (6.0 TB/s; a copy of the
+// same bytes 81 us) and 94 to 130 us with more, shorter-lived teams, which load
+// weight and bias more often than they gain; without the barriers of the
+// reductions it would take as long.  Its gradient, 16384 x 4096, takes 76 us:
+// 71 for 403 MB and 5 for the teams' sums, which is why there are few teams
+// with many rows in flight (512 teams with one row ahead: 82 us).
 #include "typed.h"
 
 #include <algorithm>
@@ -63,7 +70,7 @@ __device__ __forceinline__ void loadRow(const typename T::Stored* row, uint32_t 
     out[k] = loadPack<T>(row, (uint64_t(k) * lanes + lane) * T::kVec, cols, typename T::Stored(0.0f));
 }
 
-template <typename T, typename P, int kWaves, int kPacks>
+template <typename T, typename P, int kWaves, int kPacks, int kAhead>
 __global__ __launch_bounds__(kWaves * 64 < kTeamBlock ? kTeamBlock : kWaves * 64) void layerNormKernel(
     const typename T::Stored* x, uint64_t xStride, const typename P::Stored* weight, const typename P::Stored* bias,
     float eps, typename T::Stored* y, uint64_t yStride, float* means, float* rstds, uint64_t rows, uint32_t cols) {
@@ -78,8 +85,10 @@ __global__ __launch_bounds__(kWaves * 64 < kTeamBlock ? kTeamBlock : kWaves * 64
 
   float w[kPacks][T::kVec], b[kPacks][T::kVec];
   uint64_t row = uint64_t(blockIdx.x) * kTeams + team;
-  Pack next[kPacks];
-  if (row < rows) loadRow<T, kPacks>(x + row * xStride, lane, kLanes, cols, next);
+  Pack next[kAhead][kPacks]; // the rows that come next, the first one for the round that is due
+#pragma unroll
+  for (int n = 0; n < kAhead; ++n)
+    if (row + n * step < rows) loadRow<T, kPacks>(x + (row + n * step) * xStride, lane, kLanes, cols, next[n]);
 #pragma unroll
   for (int k = 0; k < kPacks; ++k) {
     const uint64_t c = (uint64_t(k) * kLanes + lane) * T::kVec;
@@ -88,41 +97,45 @@ __global__ __launch_bounds__(kWaves * 64 < kTeamBlock ? kTeamBlock : kWaves * 64
   }
   // every team of a work-group makes the same number of rounds (their barriers
   // are the work-group's); a team whose row is behind the last one only keeps step
-  for (uint64_t first = uint64_t(blockIdx.x) * kTeams; first < rows; first += step, row += step) {
-    const bool here = row < rows;
-    float v[kPacks][T::kVec];
-    float sum = 0.0f;
+  for (uint64_t first = uint64_t(blockIdx.x) * kTeams; first < rows;) {
 #pragma unroll
-    for (int k = 0; k < kPacks; ++k) {
-      T::unpack(next[k], v[k]);
-#pragma unroll
-      for (int i = 0; i < T::kVec; ++i) sum += v[k][i]; // elements behind the row's end are zero
-    }
-    if (row + step < rows) loadRow<T, kPacks>(x + (row + step) * xStride, lane, kLanes, cols, next);
-    const float mean = teamSum<kWaves>(here ? sum : 0.0f, lds[0], team, wave) / count;
-    float squares = 0.0f;
-#pragma unroll
-    for (int k = 0; k < kPacks; ++k) {
-      const uint32_t c = (k * kLanes + lane) * T::kVec;
-#pragma unroll
-      for (int i = 0; i < T::kVec; ++i) {
-        v[k][i] = c + i < cols ? v[k][i] - mean : 0.0f;
-        squares += v[k][i] * v[k][i];
-      }
-    }
-    const float rstd = 1.0f / sqrtf(teamSum<kWaves>(squares, lds[1], team, wave) / count + eps);
-    if (here) {
+    for (int n = 0; n < kAhead; ++n, first += step, row += step) {
+      if (n > 0 && first >= rows) break;
+      const bool here = row < rows;
+      float v[kPacks][T::kVec];
+      float sum = 0.0f;
 #pragma unroll
       for (int k = 0; k < kPacks; ++k) {
-        const uint64_t c = (uint64_t(k) * kLanes + lane) * T::kVec;
-        float out[T::kVec];
+        T::unpack(next[n][k], v[k]);
 #pragma unroll
-        for (int i = 0; i < T::kVec; ++i) out[i] = v[k][i] * rstd * w[k][i] + b[k][i];
-        storePack<T>(y + row * yStride, c, cols, out);
+        for (int i = 0; i < T::kVec; ++i) sum += v[k][i]; // elements behind the row's end are zero
       }
-      if (lane == 0) {
-        if (means != nullptr) means[row] = mean;
-        if (rstds != nullptr) rstds[row] = rstd;
+      if (row + kAhead * step < rows) loadRow<T, kPacks>(x + (row + kAhead * step) * xStride, lane, kLanes, cols, next[n]);
+      const float mean = teamSum<kWaves>(here ? sum : 0.0f, lds[0], team, wave) / count;
+      float squares = 0.0f;
+#pragma unroll
+      for (int k = 0; k < kPacks; ++k) {
+        const uint32_t c = (k * kLanes + lane) * T::kVec;
+#pragma unroll
+        for (int i = 0; i < T::kVec; ++i) {
+          v[k][i] = c + i < cols ? v[k][i] - mean : 0.0f;
+          squares += v[k][i] * v[k][i];
+        }
+      }
+      const float rstd = 1.0f / sqrtf(teamSum<kWaves>(squares, lds[1], team, wave) / count + eps);
+      if (here) {
+#pragma unroll
+        for (int k = 0; k < kPacks; ++k) {
+          const uint64_t c = (uint64_t(k) * kLanes + lane) * T::kVec;
+          float out[T::kVec];
+#pragma unroll
+          for (int i = 0; i < T::kVec; ++i) out[i] = v[k][i] * rstd * w[k][i] + b[k][i];
+          storePack<T>(y + row * yStride, c, cols, out);
+        }
+        if (lane == 0) {
+          if (means != nullptr) means[row] = mean;
+          if (rstds != nullptr) rstds[row] = rstd;
+        }
       }
     }
   }
@@ -188,7 +201,7 @@ __global__ __launch_bounds__(kLongBlock) void layerNormLongKernel(
 // ---- gradient --------------------------------------------------------------------
 
 // sums: [2][teams of the whole grid][cols] fp32, dw's before db's; null if neither is wanted
-template <typename T, typename P, int kWaves, int kPacks, bool kStats>
+template <typename T, typename P, int kWaves, int kPacks, int kAhead, bool kStats>
 __global__ __launch_bounds__(kWaves * 64 < kTeamBlock ? kTeamBlock : kWaves * 64) void layerNormGradKernel(
     const typename T::Stored* dy, uint64_t dyStride, const typename T::Stored* x, uint64_t xStride,
     const typename P::Stored* weight, const float* means, const float* rstds, float eps, typename T::Stored* dx,
@@ -205,14 +218,19 @@ __global__ __launch_bounds__(kWaves * 64 < kTeamBlock ? kTeamBlock : kWaves * 64
 
   float w[kPacks][T::kVec], dw[kPacks][T::kVec], db[kPacks][T::kVec];
   uint64_t row = uint64_t(blockIdx.x) * kTeams + team;
-  Pack nextX[kPacks], nextDy[kPacks];
+  Pack nextX[kAhead][kPacks], nextDy[kAhead][kPacks];
+  float nextMean[kAhead], nextRstd[kAhead];
+  auto load = [&](int n, uint64_t r) {
+    loadRow<T, kPacks>(x + r * xStride, lane, kLanes, cols, nextX[n]);
+    loadRow<T, kPacks>(dy + r * dyStride, lane, kLanes, cols, nextDy[n]);
+    if constexpr (!kStats) nextMean[n] = means[r], nextRstd[n] = rstds[r];
+  };
 #pragma unroll
-  for (int k = 0; k < kPacks; ++k) nextX[k] = nextDy[k] = Pack{0, 0, 0, 0};
-  float nextMean = 0.0f, nextRstd = 0.0f;
-  if (row < rows) {
-    loadRow<T, kPacks>(x + row * xStride, lane, kLanes, cols, nextX);
-    loadRow<T, kPacks>(dy + row * dyStride, lane, kLanes, cols, nextDy);
-    if constexpr (!kStats) nextMean = means[row], nextRstd = rstds[row];
+  for (int n = 0; n < kAhead; ++n) {
+#pragma unroll
+    for (int k = 0; k < kPacks; ++k) nextX[n][k] = nextDy[n][k] = Pack{0, 0, 0, 0};
+    nextMean[n] = nextRstd[n] = 0.0f;
+    if (row + n * step < rows) load(n, row + n * step);
   }
 #pragma unroll
   for (int k = 0; k < kPacks; ++k) {
@@ -221,62 +239,62 @@ __global__ __launch_bounds__(kWaves * 64 < kTeamBlock ? kTeamBlock : kWaves * 64
     for (int i = 0; i < T::kVec; ++i) dw[k][i] = db[k][i] = 0.0f;
   }
   int round = 0;
-  for (uint64_t first = uint64_t(blockIdx.x) * kTeams; first < rows; first += step, row += step, round ^= 1) {
-    const bool here = row < rows;
-    float h[kPacks][T::kVec], g[kPacks][T::kVec];
-    float mean = nextMean, rstd = nextRstd;
+  for (uint64_t first = uint64_t(blockIdx.x) * kTeams; first < rows;) {
 #pragma unroll
-    for (int k = 0; k < kPacks; ++k) {
-      T::unpack(nextX[k], h[k]);
-      T::unpack(nextDy[k], g[k]);
-    }
-    if (row + step < rows) {
-      loadRow<T, kPacks>(x + (row + step) * xStride, lane, kLanes, cols, nextX);
-      loadRow<T, kPacks>(dy + (row + step) * dyStride, lane, kLanes, cols, nextDy);
-      if constexpr (!kStats) nextMean = means[row + step], nextRstd = rstds[row + step];
-    }
-    if constexpr (kStats) {
-      float sum = 0.0f, squares = 0.0f;
+    for (int n = 0; n < kAhead; ++n, first += step, row += step, round ^= 1) {
+      if (n > 0 && first >= rows) break;
+      const bool here = row < rows;
+      float h[kPacks][T::kVec], g[kPacks][T::kVec];
+      float mean = nextMean[n], rstd = nextRstd[n];
+#pragma unroll
+      for (int k = 0; k < kPacks; ++k) {
+        T::unpack(nextX[n][k], h[k]);
+        T::unpack(nextDy[n][k], g[k]);
+      }
+      if (row + kAhead * step < rows) load(n, row + kAhead * step);
+      if constexpr (kStats) {
+        float sum = 0.0f, squares = 0.0f;
+#pragma unroll
+        for (int k = 0; k < kPacks; ++k)
+#pragma unroll
+          for (int i = 0; i < T::kVec; ++i) sum += h[k][i];
+        mean = teamSum<kWaves>(sum, lds[0], team, wave) / count;
+#pragma unroll
+        for (int k = 0; k < kPacks; ++k) {
+          const uint32_t c = (k * kLanes + lane) * T::kVec;
+#pragma unroll
+          for (int i = 0; i < T::kVec; ++i) {
+            const float d = c + i < cols ? h[k][i] - mean : 0.0f;
+            squares += d * d;
+          }
+        }
+        rstd = 1.0f / sqrtf(teamSum<kWaves>(squares, lds[1], team, wave) / count + eps);
+      }
+      Float2 s{0.0f, 0.0f};
 #pragma unroll
       for (int k = 0; k < kPacks; ++k)
 #pragma unroll
-        for (int i = 0; i < T::kVec; ++i) sum += h[k][i];
-      mean = teamSum<kWaves>(sum, lds[0], team, wave) / count;
-#pragma unroll
-      for (int k = 0; k < kPacks; ++k) {
-        const uint32_t c = (k * kLanes + lane) * T::kVec;
-#pragma unroll
         for (int i = 0; i < T::kVec; ++i) {
-          const float d = c + i < cols ? h[k][i] - mean : 0.0f;
-          squares += d * d;
+          // behind the row's end dy is zero, so that whatever h is there counts for nothing
+          h[k][i] = (h[k][i] - mean) * rstd;
+          if (here) {
+            dw[k][i] += g[k][i] * h[k][i];
+            db[k][i] += g[k][i];
+          }
+          g[k][i] *= w[k][i];
+          s.x += g[k][i];
+          s.y += g[k][i] * h[k][i];
         }
-      }
-      rstd = 1.0f / sqrtf(teamSum<kWaves>(squares, lds[1], team, wave) / count + eps);
-    }
-    Float2 s{0.0f, 0.0f};
+      s = teamSum2<kWaves>(s, lds2[round], team, wave);
+      const float alongOnes = s.x / count, alongH = s.y / count;
+      if (here && dx != nullptr) {
 #pragma unroll
-    for (int k = 0; k < kPacks; ++k)
+        for (int k = 0; k < kPacks; ++k) {
+          float out[T::kVec];
 #pragma unroll
-      for (int i = 0; i < T::kVec; ++i) {
-        // behind the row's end dy is zero, so that whatever h is there counts for nothing
-        h[k][i] = (h[k][i] - mean) * rstd;
-        if (here) {
-          dw[k][i] += g[k][i] * h[k][i];
-          db[k][i] += g[k][i];
+          for (int i = 0; i < T::kVec; ++i) out[i] = rstd * (g[k][i] - alongOnes - h[k][i] * alongH);
+          storePack<T>(dx + row * dxStride, (uint64_t(k) * kLanes + lane) * T::kVec, cols, out);
         }
-        g[k][i] *= w[k][i];
-        s.x += g[k][i];
-        s.y += g[k][i] * h[k][i];
-      }
-    s = teamSum2<kWaves>(s, lds2[round], team, wave);
-    const float alongOnes = s.x / count, alongH = s.y / count;
-    if (here && dx != nullptr) {
-#pragma unroll
-      for (int k = 0; k < kPacks; ++k) {
-        float out[T::kVec];
-#pragma unroll
-        for (int i = 0; i < T::kVec; ++i) out[i] = rstd * (g[k][i] - alongOnes - h[k][i] * alongH);
-        storePack<T>(dx + row * dxStride, (uint64_t(k) * kLanes + lane) * T::kVec, cols, out);
       }
     }
   }
@@ -309,6 +327,7 @@ __global__ __launch_bounds__(1024) void layerNormParamKernel(const float* sums, 
   float sum = 0.0f;
   if (c < cols) {
     const float* from = sums + (second ? teams * cols : 0) + c;
+#pragma unroll 8
     for (uint64_t t = wave; t < teams; t += 16) sum += from[t * cols];
   }
   lds[wave][lane] = sum;
@@ -427,13 +446,12 @@ unsigned gridFor(uint64_t rows, uint64_t teamsPerGroup, uint64_t most) {
   return static_cast<unsigned>(std::min((rows + teamsPerGroup - 1) / teamsPerGroup, most));
 }
 
-template <typename T, typename P, int kWaves, int kPacks>
+template <typename T, typename P, int kWaves, int kPacks, int kAhead, int kPerCu>
 int launchNorm(polar_hip_device* dev, const NormArgs& a) {
   constexpr int kBlock = kWaves * 64 < kTeamBlock ? kTeamBlock : kWaves * 64;
   constexpr int kTeams = kBlock / (kWaves * 64);
-  // as many work-groups as are resident at once (12 to 16 waves per CU)
-  const uint64_t most = uint64_t(dev->info.compute_units) * (kBlock >= 1024 ? 1 : kBlock >= 512 ? 2 : 4);
-  POLAR_HIP_TRY(launchKernel(dev, layerNormKernel<T, P, kWaves, kPacks>, dim3(gridFor(a.rows, kTeams, most)), dim3(kBlock),
+  const uint64_t most = uint64_t(dev->info.compute_units) * kPerCu; // work-groups
+  POLAR_HIP_TRY(launchKernel(dev, layerNormKernel<T, P, kWaves, kPacks, kAhead>, dim3(gridFor(a.rows, kTeams, most)), dim3(kBlock),
                              static_cast<const typename T::Stored*>(a.x), a.xStride,
                              static_cast<const typename P::Stored*>(a.weight),
                              static_cast<const typename P::Stored*>(a.bias), a.eps,
@@ -444,12 +462,16 @@ int launchNorm(polar_hip_device* dev, const NormArgs& a) {
 
 template <typename T, typename P> int norm(polar_hip_device* dev, const NormArgs& a) {
   const uint64_t wavePacks = (a.cols + 64 * T::kVec - 1) / (64 * T::kVec); // packs of a wave that a row fills
-  if (wavePacks <= 1) return launchNorm<T, P, 1, 1>(dev, a);
-  if (wavePacks <= 2) return launchNorm<T, P, 1, 2>(dev, a);
-  if (wavePacks <= 4) return launchNorm<T, P, 4, 1>(dev, a);
-  if (wavePacks <= 8) return launchNorm<T, P, 4, 2>(dev, a);
-  if (wavePacks <= 16) return launchNorm<T, P, 8, 2>(dev, a);
-  if (wavePacks <= 32) return launchNorm<T, P, 16, 2>(dev, a);
+  // waves per row, packs per lane, rows ahead, work-groups per CU: the fastest of those tried
+  // with bf16 rows as long as each line allows (268 MB in and 268 out: 2 waves of 2 packs 48.5
+  // us, 4 of 1 53.5; 4 of 2 49.0, 8 of 1 50.6; 8 of 2 with four rows ahead 88.7 for twice
+  // that, with one and two groups 90.7, 4 of 4 95)
+  if (wavePacks <= 1) return launchNorm<T, P, 1, 1, 1, 6>(dev, a);
+  if (wavePacks <= 2) return launchNorm<T, P, 1, 2, 1, 6>(dev, a);
+  if (wavePacks <= 4) return launchNorm<T, P, 2, 2, 1, 6>(dev, a);
+  if (wavePacks <= 8) return launchNorm<T, P, 4, 2, 1, 4>(dev, a);
+  if (wavePacks <= 16) return launchNorm<T, P, 8, 2, 4, 1>(dev, a);
+  if (wavePacks <= 32) return launchNorm<T, P, 16, 2, 1, 1>(dev, a);
   POLAR_HIP_TRY(launchKernel(dev, layerNormLongKernel<T, P>, dim3(gridFor(a.rows, 1, 1u << 20)), dim3(kLongBlock),
                              static_cast<const typename T::Stored*>(a.x), a.xStride,
                              static_cast<const typename P::Stored*>(a.weight),
@@ -466,13 +488,12 @@ int launchParams(polar_hip_device* dev, const NormGradArgs& a, const float* sums
   return POLAR_HIP_OK;
 }
 
-template <typename T, typename P, int kWaves, int kPacks>
+template <typename T, typename P, int kWaves, int kPacks, int kAhead, int kPerCu>
 int launchNormGrad(polar_hip_device* dev, const NormGradArgs& a) {
   constexpr int kBlock = kWaves * 64 < kTeamBlock ? kTeamBlock : kWaves * 64;
   constexpr int kTeams = kBlock / (kWaves * 64);
   const bool params = a.dweight != nullptr || a.dbias != nullptr;
-  const uint64_t most = uint64_t(dev->info.compute_units) * (kBlock >= 512 ? 1 : 2);
-  const unsigned grid = gridFor(a.rows, kTeams, most);
+  const unsigned grid = gridFor(a.rows, kTeams, uint64_t(dev->info.compute_units) * kPerCu);
   const uint64_t teams = uint64_t(grid) * kTeams;
   std::lock_guard<std::mutex> lock(dev->workspaceMu);
   void* area = nullptr;
@@ -480,8 +501,8 @@ int launchNormGrad(polar_hip_device* dev, const NormGradArgs& a) {
     const int st = workspaceFor(dev, 2 * teams * a.cols * sizeof(float), &area);
     if (st != POLAR_HIP_OK) return st;
   }
-  auto kernel = a.mean == nullptr ? layerNormGradKernel<T, P, kWaves, kPacks, true>
-                                  : layerNormGradKernel<T, P, kWaves, kPacks, false>;
+  auto kernel = a.mean == nullptr ? layerNormGradKernel<T, P, kWaves, kPacks, kAhead, true>
+                                  : layerNormGradKernel<T, P, kWaves, kPacks, kAhead, false>;
   POLAR_HIP_TRY(launchKernel(dev, kernel, dim3(grid), dim3(kBlock), static_cast<const typename T::Stored*>(a.dy),
                              a.dyStride, static_cast<const typename T::Stored*>(a.x), a.xStride,
                              static_cast<const typename P::Stored*>(a.weight), a.mean, a.rstd, a.eps,
@@ -518,12 +539,17 @@ template <typename T, typename P> int launchLongGrad(polar_hip_device* dev, cons
 
 template <typename T, typename P> int normGrad(polar_hip_device* dev, const NormGradArgs& a) {
   const uint64_t wavePacks = (a.cols + 64 * T::kVec - 1) / (64 * T::kVec);
-  if (wavePacks <= 1) return launchNormGrad<T, P, 1, 1>(dev, a);
-  if (wavePacks <= 2) return launchNormGrad<T, P, 1, 2>(dev, a);
-  if (wavePacks <= 4) return launchNormGrad<T, P, 4, 1>(dev, a);
-  if (wavePacks <= 8) return launchNormGrad<T, P, 4, 2>(dev, a);
-  if (wavePacks <= 16) return launchNormGrad<T, P, 8, 2>(dev, a);
-  if (wavePacks <= 32) return launchNormGrad<T, P, 16, 2>(dev, a);
+  // as above; two groups of four waves per CU, or one of eight or more, as each team adds
+  // its sums to what the second kernel reads (16384 x 4096: 8 waves of 1 pack with four rows
+  // ahead 75.5 us, 4 of 2 with one 82, twice the groups 84; 32768 x 2048: 4 waves of 1 with two
+  // rows ahead and two groups 76.9, one group 105; 65536 x 1024: 1 wave of 2 with three ahead
+  // 78.9, one 85.7)
+  if (wavePacks <= 1) return launchNormGrad<T, P, 1, 1, 3, 2>(dev, a);
+  if (wavePacks <= 2) return launchNormGrad<T, P, 1, 2, 3, 2>(dev, a);
+  if (wavePacks <= 4) return launchNormGrad<T, P, 4, 1, 2, 2>(dev, a);
+  if (wavePacks <= 8) return launchNormGrad<T, P, 8, 1, 4, 1>(dev, a);
+  if (wavePacks <= 16) return launchNormGrad<T, P, 8, 2, 2, 1>(dev, a);
+  if (wavePacks <= 32) return launchNormGrad<T, P, 8, 4, 1, 1>(dev, a); // 16 waves would have 128 registers each, and spill
   return launchLongGrad<T, P>(dev, a);
 }
 
