@@ -154,6 +154,18 @@ __device__ __forceinline__ uint32_t randomBits(uint32_t seed, uint64_t element) 
   return h ^ (h >> 16);
 }
 
+// The square root, rounded to nearest: the hardware's is good to a unit in the last
+// place, and the sign of what its two neighbours leave over says which of the three it
+// is.  Exact where that rest is a normal number (v from 2^-96 on), else as the hardware
+// has it; 0, infinity and NaN stay what they are.
+__device__ __forceinline__ float rootOf(float v) {
+  const float r = __builtin_amdgcn_sqrtf(v);
+  const float below = __builtin_bit_cast(float, __builtin_bit_cast(uint32_t, r) - 1u);
+  const float above = __builtin_bit_cast(float, __builtin_bit_cast(uint32_t, r) + 1u);
+  float root = __builtin_fmaf(-below, r, v) <= 0.0f ? below : r;
+  return __builtin_fmaf(-above, r, v) > 0.0f ? above : root;
+}
+
 // Four consecutive elements of a tensor in a lane, `n` of them (0 .. 4) real.  P: the
 // parameter's type; one of 16 bits is a copy of the fp32 master.  G: the gradient's.
 template <typename P, typename G, bool kSmall> struct Four {
@@ -187,12 +199,12 @@ template <typename P, typename G, bool kSmall> struct Four {
       v[i] = v[i] * t.beta2 + (g[i] * g[i]) * t.rest2;
       const float scaled = m[i] * t.stepSize;
       if constexpr (kSmall) {
-        // the hardware's square root and reciprocal, each good to a unit in the last place: against states
-        // of three bits and a parameter that the quotient changes by a thousandth that is nothing, and the
-        // exact sequences' 20 instructions per element would set the time (788 us for 260 million elements
-        // instead of 708).  The divisor is 0, or far above the subnormal numbers: a root's smallest value
-        // is 3.7e-23.
-        r[i] = __builtin_amdgcn_sqrtf(v[i]);
+        // The quotient only moves the parameter, by a thousandth or so of its size: the hardware's
+        // reciprocal, good to a unit in the last place, is nothing against the three bits that the
+        // states have.  (The divisor is 0, or far above the subnormal numbers: a root's smallest
+        // value is 3.7e-23.)  With the exact division and sqrtf their 20 instructions more per
+        // element would set the time: 788 us for 260 million elements.
+        r[i] = rootOf(v[i]);
         p[i] = (p[i] - p[i] * decay) - scaled * __builtin_amdgcn_rcpf(r[i] * t.byCorrection + t.eps);
       } else {
         r[i] = sqrtf(v[i]);
