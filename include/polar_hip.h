@@ -382,7 +382,8 @@ int polar_hip_flogprob(polar_hip_device* dev, int type, const void* logits,
                        uint64_t rows, uint64_t cols);
 /* flogprob_grad: dlogits from the gradients with regard to logprob and entropy
  * (either may be null: zeros).  stats, and entropy where dentropy is given, come
- * from flogprob with the same logits and scale.  A row whose token is negative
+ * from flogprob with the same logits and scale; stats may be null, at the price
+ * of reading the logits once more to compute them (rows up to 2^24).  A row whose token is negative
  * has no share of dlogprob, a row of -infinity alone gets zeros, a row whose token
  * is >= cols NaN.  dlogits may be logits (equal strides). */
 int polar_hip_flogprob_grad(polar_hip_device* dev, int type, const void* logits,

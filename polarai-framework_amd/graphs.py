@@ -1,4 +1,4 @@
-"""Kernel DAGs of the two model configurations, built the way the framework
+"""Kernel DAGs of the two model configurations and of a language model's head, built the way the framework
 builds them, for the mini-executor.
 
 `Graph` mirrors what the framework's graph front-end hands to its compiler:
@@ -90,6 +90,21 @@ class Graph:
         m = a.shape[1] if ta else a.shape[0]
         n = b.shape[0] if tb else b.shape[1]
         return self._op(f"fmatmul_{'t' if ta else 'f'}_{'t' if tb else 'f'}", [a, b], (m, n), name)
+
+    def layernorm(self, x, params, eps=1e-5, name=""):
+        return self._op("flayernorm", [x, params, eps], x.shape, name)
+
+    def layernorm_grad(self, grad, x, params, eps=1e-5, name=""):
+        return self._op("flayernorm_grad", [grad, x, params, eps], x.shape, name)
+
+    def layernorm_grad_params(self, grad, x, eps=1e-5, name=""):
+        return self._op("flayernorm_grad_params", [grad, x, eps], (2, x.shape[1]), name)
+
+    def logprob(self, logits, tokens, scale=1.0, name=""):
+        return self._op("flogprob", [logits, tokens, scale], (logits.shape[0],), name)
+
+    def logprob_grad(self, logits, tokens, grad, scale=1.0, name=""):
+        return self._op("flogprob_grad", [logits, tokens, grad, scale], logits.shape, name)
 
     def clusters(self):
         top = max(n.level for n in self.nodes)
@@ -193,3 +208,30 @@ def mlp_graphs(x, w1, w2, y, learning_rate=-0.01):
     named = dict(X=X, W1=W1, W2=W2, Y=Y, A1=a1, H=h, A2=a2, P=p, L=loss,
                  gP=g_p, gA2=g_a2, gH=g_h, gW2=g_w2, gA1=g_a1, gW1=g_w1)
     return f, g, u, named
+
+
+def token_head_graphs(x, norm, w, tokens, learning_rate=-0.01):
+    """The head of a language model: Y = layer norm of X with `norm` (weight and bias, 2 x columns), Z = Y W, L = log
+    probabilities of `tokens` (one per row; negative: the row does not count); then the gradient graph of the negative mean
+    of L -- textbook derivatives, unlike mlp_graphs, as the reference has no such operators -- and the weight-changing graph.
+    Returns (forward, gradient, update, named values)."""
+    tokens = np.asarray(tokens)
+    f = Graph("head_forward")
+    X, N, W, T = f.input(x, "X"), f.input(norm, "N"), f.input(w, "W"), f.input(tokens, "T")
+    y = f.layernorm(X, N, name="Y")
+    z = f.matmul(y, W, name="Z")
+    logp = f.logprob(z, T, name="L")
+
+    g = Graph("head_gradient")
+    seed = g.constant(-1.0 / max(1, int((tokens >= 0).sum())), logp.shape, "seed")
+    g_z = g.logprob_grad(g.holder(z), g.holder(T), seed, name="gZ")
+    g_w = g.matmul(g.holder(y), g_z, ta=True, name="gW")
+    g_y = g.matmul(g_z, g.holder(W), tb=True, name="gY")
+    g_n = g.layernorm_grad_params(g_y, g.holder(X), name="gN")
+    g_x = g.layernorm_grad(g_y, g.holder(X), g.holder(N), name="gX")
+
+    u = Graph("head_update")
+    for value, grad, tag in ((W, g_w, "W"), (N, g_n, "N")):
+        step = u.mul(u.holder(grad), u.constant(learning_rate, grad.shape, "lr_" + tag), name="step_" + tag)
+        u.add(step, u.holder(value), name="new_" + tag, into=value)
+    return f, g, u, dict(X=X, N=N, W=W, T=T, Y=y, Z=z, L=logp, gZ=g_z, gW=g_w, gY=g_y, gN=g_n, gX=g_x)

@@ -291,6 +291,33 @@ class Harness:
         self.node(f"fmatmul_{'t' if ta else 'f'}_{'t' if tb else 'f'}", [a, b, out], 2)
         return out
 
+    # operators of a language model's training step; weight and bias of a norm are the two rows of `params`,
+    # tokens are whole numbers in fp32
+    def flayernorm(self, x, params, eps=1e-5, out=None):
+        out = out or self.tensor(*x.shape)
+        self.node("flayernorm", [x, params, float(eps), out], 3)
+        return out
+
+    def flayernorm_grad(self, grad, x, params, eps=1e-5, out=None):
+        out = out or self.tensor(*x.shape)
+        self.node("flayernorm_grad", [grad, x, params, float(eps), out], 4)
+        return out
+
+    def flayernorm_grad_params(self, grad, x, eps=1e-5, out=None):
+        out = out or self.tensor(2, x.shape[1])
+        self.node("flayernorm_grad_params", [grad, x, float(eps), out], 3)
+        return out
+
+    def flogprob(self, logits, tokens, scale=1.0, out=None):
+        out = out or self.tensor(logits.shape[0])
+        self.node("flogprob", [logits, tokens, float(scale), out], 3)
+        return out
+
+    def flogprob_grad(self, logits, tokens, grad, scale=1.0, out=None):
+        out = out or self.tensor(*logits.shape)
+        self.node("flogprob_grad", [logits, tokens, grad, float(scale), out], 4)
+        return out
+
     # -- allocator access for protocol tests --------------------------------
     def allocate(self, t, device=0):
         self._ok(self.lib.polar_harness_allocate(self.h, t.vaddr, device), "allocate")

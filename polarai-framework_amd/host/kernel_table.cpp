@@ -277,6 +277,102 @@ void launchMatMulAddSigmoid(HipDevice& d, BackendAllocator& al, LaunchCommand& c
               cmd.nativeKernelName);
 }
 
+// Operators of a language model's training step.  The framework launches a node
+// for one result tensor (every other tensor argument is locked READ), so each of
+// these computes one: statistics are computed again where the C ABI could take
+// them from the forward pass, weight and bias of a norm are the two rows of one
+// tensor, tokens are fp32 whole numbers like every tensor here.
+void check2D(const LaunchCommand& cmd, const TensorArg& t) {
+  if (t.info->dims != 2) fatal("%s: tensor %zu must be 2-D", cmd.nativeKernelName, t.record.virtualAddress);
+}
+void checkShape(const LaunchCommand& cmd, const TensorArg& t, uint64_t rows, uint64_t cols) {
+  check2D(cmd, t);
+  if (t.info->shape[0] != rows || t.info->shape[1] != cols)
+    fatal("%s: tensor %zu is %llux%llu, %llux%llu needed", cmd.nativeKernelName, t.record.virtualAddress,
+          (unsigned long long)t.info->shape[0], (unsigned long long)t.info->shape[1], (unsigned long long)rows,
+          (unsigned long long)cols);
+}
+void checkCount(const LaunchCommand& cmd, const TensorArg& t, uint64_t count) {
+  if (t.count != count)
+    fatal("%s: tensor %zu holds %llu elements, %llu needed", cmd.nativeKernelName, t.record.virtualAddress,
+          (unsigned long long)t.count, (unsigned long long)count);
+}
+
+// flayernorm: [0]x T (2-D) [1]weight and bias T (2 x columns) [2]eps D [3]out T
+void launchLayerNorm(HipDevice& d, BackendAllocator& al, LaunchCommand& cmd) {
+  TensorArg x = tensorArg(cmd, 0), wb = tensorArg(cmd, 1), out = tensorArg(cmd, 3);
+  const float eps = scalarArg(cmd, 2);
+  check2D(cmd, x);
+  const uint64_t rows = x.info->shape[0], cols = x.info->shape[1];
+  checkShape(cmd, wb, 2, cols);
+  checkShape(cmd, out, rows, cols);
+  float* weight = d.resolve(al, wb.record);
+  checkStatus(polar_hip_flayernorm(d.native(), POLAR_HIP_F32, d.resolve(al, x.record), cols, POLAR_HIP_F32, weight,
+                                   weight + cols, eps, d.resolve(al, out.record), cols, nullptr, nullptr, rows, cols),
+              "polar_hip_flayernorm");
+}
+
+// flayernorm_grad: [0]gradient T [1]x T [2]weight and bias T (2 x columns) [3]eps D [4]out T: the gradient
+// with regard to x
+void launchLayerNormGrad(HipDevice& d, BackendAllocator& al, LaunchCommand& cmd) {
+  TensorArg dy = tensorArg(cmd, 0), x = tensorArg(cmd, 1), wb = tensorArg(cmd, 2), out = tensorArg(cmd, 4);
+  const float eps = scalarArg(cmd, 3);
+  check2D(cmd, x);
+  const uint64_t rows = x.info->shape[0], cols = x.info->shape[1];
+  checkShape(cmd, dy, rows, cols);
+  checkShape(cmd, wb, 2, cols);
+  checkShape(cmd, out, rows, cols);
+  checkStatus(polar_hip_flayernorm_grad(d.native(), POLAR_HIP_F32, d.resolve(al, dy.record), cols,
+                                        d.resolve(al, x.record), cols, POLAR_HIP_F32, d.resolve(al, wb.record), nullptr,
+                                        nullptr, eps, d.resolve(al, out.record), cols, nullptr, nullptr, rows, cols),
+              "polar_hip_flayernorm_grad");
+}
+
+// flayernorm_grad_params: [0]gradient T [1]x T [2]eps D [3]out T (2 x columns): the gradients with regard to
+// weight and bias
+void launchLayerNormGradParams(HipDevice& d, BackendAllocator& al, LaunchCommand& cmd) {
+  TensorArg dy = tensorArg(cmd, 0), x = tensorArg(cmd, 1), out = tensorArg(cmd, 3);
+  const float eps = scalarArg(cmd, 2);
+  check2D(cmd, x);
+  const uint64_t rows = x.info->shape[0], cols = x.info->shape[1];
+  checkShape(cmd, dy, rows, cols);
+  checkShape(cmd, out, 2, cols);
+  float* weight = d.resolve(al, out.record);
+  checkStatus(polar_hip_flayernorm_grad(d.native(), POLAR_HIP_F32, d.resolve(al, dy.record), cols,
+                                        d.resolve(al, x.record), cols, POLAR_HIP_F32, nullptr, nullptr, nullptr, eps,
+                                        nullptr, cols, weight, weight + cols, rows, cols),
+              "polar_hip_flayernorm_grad");
+}
+
+// flogprob: [0]logits T (2-D) [1]tokens T (one per row) [2]scale D [3]out T (one per row)
+void launchLogProb(HipDevice& d, BackendAllocator& al, LaunchCommand& cmd) {
+  TensorArg x = tensorArg(cmd, 0), tokens = tensorArg(cmd, 1), out = tensorArg(cmd, 3);
+  const float scale = scalarArg(cmd, 2);
+  check2D(cmd, x);
+  const uint64_t rows = x.info->shape[0], cols = x.info->shape[1];
+  checkCount(cmd, tokens, rows);
+  checkCount(cmd, out, rows);
+  checkStatus(polar_hip_flogprob(d.native(), POLAR_HIP_F32, d.resolve(al, x.record), cols, POLAR_HIP_INDEX_F32,
+                                 d.resolve(al, tokens.record), scale, d.resolve(al, out.record), nullptr, nullptr, 0,
+                                 nullptr, nullptr, rows, cols),
+              "polar_hip_flogprob");
+}
+
+// flogprob_grad: [0]logits T (2-D) [1]tokens T (one per row) [2]gradient T (one per row) [3]scale D [4]out T
+void launchLogProbGrad(HipDevice& d, BackendAllocator& al, LaunchCommand& cmd) {
+  TensorArg x = tensorArg(cmd, 0), tokens = tensorArg(cmd, 1), g = tensorArg(cmd, 2), out = tensorArg(cmd, 4);
+  const float scale = scalarArg(cmd, 3);
+  check2D(cmd, x);
+  const uint64_t rows = x.info->shape[0], cols = x.info->shape[1];
+  checkCount(cmd, tokens, rows);
+  checkCount(cmd, g, rows);
+  checkShape(cmd, out, rows, cols);
+  checkStatus(polar_hip_flogprob_grad(d.native(), POLAR_HIP_F32, d.resolve(al, x.record), cols, POLAR_HIP_INDEX_F32,
+                                      d.resolve(al, tokens.record), scale, nullptr, d.resolve(al, g.record), nullptr,
+                                      nullptr, d.resolve(al, out.record), cols, rows, cols),
+              "polar_hip_flogprob_grad");
+}
+
 struct TableEntry {
   const char* name;
   Launcher fn;
@@ -311,6 +407,11 @@ const TableEntry kTable[] = {
     {"fmatmul_f_t_fadd_fsigmoid", launchMatMulAddSigmoid<false, true>},
     {"fmatmul_t_f_fadd_fsigmoid", launchMatMulAddSigmoid<true, false>},
     {"fmatmul_t_t_fadd_fsigmoid", launchMatMulAddSigmoid<true, true>},
+    {"flayernorm", launchLayerNorm},
+    {"flayernorm_grad", launchLayerNormGrad},
+    {"flayernorm_grad_params", launchLayerNormGradParams},
+    {"flogprob", launchLogProb},
+    {"flogprob_grad", launchLogProbGrad},
 };
 
 } // namespace

@@ -405,6 +405,25 @@ def test_logprob_grad(dev, rows, cols, kind):
         t.free()
 
 
+@pytest.mark.parametrize("rows,cols,kind", [(1, 5, "f32"), (3, 70001, "bf16"), (700, 129, "f16"), (2, 300007, "f32")])
+def test_logprob_grad_computes_missing_stats(dev, rows, cols, kind):
+    """Without the forward pass's stats the same bits come out."""
+    _say("flogprob_grad without stats", rows, cols, kind)
+    rng = np.random.default_rng(cols)
+    x = ref.rounded(rng.standard_normal((rows, cols)) * 2, kind)
+    X, T = Matrix(dev, kind, rows, cols, cols + 1, 1, x), Raw(dev, rng.integers(-1, cols, rows).astype(np.int64))
+    S, H, G = Raw(dev, np.zeros((rows, 2), np.float32)), Raw(dev, np.zeros(rows, np.float32)), Raw(dev, np.full(rows, -0.5, np.float32))
+    one, other = Matrix(dev, kind, rows, cols), Matrix(dev, kind, rows, cols)
+    a = dict(dtype=kind, stride=X.stride, scale=1.5)
+    dev.flogprob(X, None, None, rows, cols, stats=S, entropy=H, **a)
+    for entropy in (None, H):
+        dev.flogprob_grad(X, T, S, G, one, rows, cols, entropy=entropy, dentropy=entropy and G, **a)
+        dev.flogprob_grad(X, T, None, G, other, rows, cols, entropy=entropy, dentropy=entropy and G, **a)
+        assert np.array_equal(one.values(), other.values())
+    for t in (X, T, S, H, G, one, other):
+        t.free()
+
+
 def test_logprob_of_more_rows_than_a_launch_takes(dev):
     """One logit per row: log probability and gradient are 0; more work-groups than one launch has."""
     _say("flogprob 8.5 million rows")

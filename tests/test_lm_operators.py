@@ -79,7 +79,7 @@ def test_logprob_refuses(lib, handle, change, words):
 
 @pytest.mark.parametrize("change,words", [
     (dict(dev=0), "dev is null"), (dict(type=3), "element type"), (dict(tokenType=-1), "token type"), (dict(cols=0), "rows of 1"),
-    (dict(scale=0.0), "scale"), (dict(stats=0), "null"), (dict(dlogits=0), "null"), (dict(logits=0), "null"),
+    (dict(scale=0.0), "scale"), (dict(dlogits=0), "null"), (dict(logits=0), "null"),
     (dict(tokens=0), "tokens"), (dict(entropy=0), "entropy"), (dict(stride=7), "stride"), (dict(dlogitsStride=7), "stride"),
     (dict(dlogits=A, dlogitsStride=9), "in place"), (dict(dlogits=A + 1), "misaligned")])
 def test_logprob_grad_refuses(lib, handle, change, words):
@@ -168,3 +168,23 @@ def test_logprob_gradient_formula_against_differences():
 def test_8_bit_floats_of_the_reference():
     assert ref.E4M3[0x7E] == 448 and ref.E4M3[0x08] == 2.0 ** -6 and ref.E4M3[1] == 2.0 ** -9 and ref.E4M3[0xB8] == -1.0
     assert np.all(np.diff(ref.E4M3[:0x7F]) > 0)
+
+
+def test_token_head_graphs_call_sequence_on_the_mock_device():
+    """Forward, gradient and update graphs of a model head: each launch reaches the device with the operands in order."""
+    from polarai_framework_amd import graphs, harness
+    x, norm, w = np.ones((3, 4)), np.ones((2, 4)), np.ones((4, 5))
+    f, g, u, named = graphs.token_head_graphs(x, norm, w, np.array([1, -1, 4]))
+    assert [n.kernel for n in f.nodes if n.kind == "op"] == ["flayernorm", "fmatmul_f_f", "flogprob"]
+    assert [n.kernel for n in g.nodes if n.kind == "op"] == ["flogprob_grad", "fmatmul_t_f", "fmatmul_f_t",
+                                                             "flayernorm_grad_params", "flayernorm_grad"]
+    seed = [n for n in g.nodes if n.name == "seed"][0]
+    assert seed.shape == (3,) and np.all(seed.data == np.float32(-0.5))
+    assert named["gN"].shape == (2, 4) and named["gW"].shape == (4, 5) and named["gX"].shape == (3, 4)
+    with harness.Harness(plugin=None) as h:
+        tensors = {}
+        for gr in (f, g, u):
+            graphs.emit(gr, h, tensors)
+            h.run()
+            h.clear_program()
+        assert h.counters().launches == 3 + 5 + 4
