@@ -361,7 +361,7 @@ int polar_hip_flayernorm_grad(polar_hip_device* dev, int type, const void* dy,
 
 #define POLAR_HIP_LOGPROB_MAX_TOP 32
 /* flogprob: for each row of logits (1 to 2^24 of them), of the distribution
- * softmax(scale * logits), scale > 0:
+ * softmax(scale * logits), scale from 2^-64 to 2^64:
  *   logprob[row]  log probability of tokens[row]; 0 where the token is negative
  *                 (a place that does not count), NaN where it is >= cols
  *   stats[row]    two values that flogprob_grad wants: the largest logit, and the
@@ -370,7 +370,8 @@ int polar_hip_flayernorm_grad(polar_hip_device* dev, int type, const void* dy,
  *   entropy[row]  -sum p log p
  *   topIndex, topLogprob [row][top]  the `top` (0 to 32, at most cols) likeliest
  *                 tokens in order, of equal logits the lowest first, and their
- *                 log probabilities
+ *                 log probabilities (-infinity for those that are ruled out, where
+ *                 no others are left)
  * Each output may be null (topIndex and topLogprob where top is 0).  -infinity
  * is a logit that is ruled out.  A row of nothing else: log probabilities
  * -infinity, entropy 0, stats both -infinity.  A row with a NaN or +infinity:
@@ -423,7 +424,8 @@ typedef struct polar_hip_adamw_config {
  *   param = param - lr weight_decay param
  *           - lr / (1 - beta1^step) m / (sqrt(v) / sqrt(1 - beta2^step) + eps)
  * The list is read before the call returns.  All of it is checked before
- * anything is launched.  Tensors must not overlap.  8-bit states are rounded
+ * anything is launched.  Tensors must not overlap (parameters that do are
+ * refused: weights that two layers share are listed once).  8-bit states are rounded
  * stochastically, up where the upper (v) or lower (m) 16 bits of a hash of seed
  * and element number say so; a block whose scale is not above 2^-100 holds zeros,
  * and a state that is not finite is held as NaN, without a say in its block's

@@ -27,6 +27,9 @@
 
 #include <algorithm>
 #include <cmath>
+#include <new>
+#include <utility>
+#include <vector>
 
 using namespace polar_hip_detail;
 
@@ -332,6 +335,23 @@ int polar_hip_fadamw(polar_hip_device* dev, const polar_hip_adamw_config* config
                           (!copy || alignedTo(t.master, 4)) && (small || (alignedTo(t.m, 4) && alignedTo(t.v, 4))) &&
                           (!small || (alignedTo(t.m_scale, 4) && alignedTo(t.v_scale, 4))),
                       "misaligned pointer");
+  }
+  // a parameter that is listed twice (weights that two layers share) would be updated by two work-groups at once
+  if (count > 1) {
+    try {
+      std::vector<std::pair<uintptr_t, uintptr_t>> spans;
+      spans.reserve(count);
+      for (uint64_t i = 0; i < count; ++i) {
+        const uintptr_t at = reinterpret_cast<uintptr_t>(tensors[i].param);
+        if (tensors[i].count != 0) spans.emplace_back(at, at + tensors[i].count * sizeOf(config->param_type));
+      }
+      std::sort(spans.begin(), spans.end());
+      for (size_t i = 1; i < spans.size(); ++i)
+        POLAR_HIP_REQUIRE(spans[i - 1].second <= spans[i].first, "two tensors' parameters overlap");
+    } catch (const std::bad_alloc&) {
+      return fail(POLAR_HIP_ERR_OOM, "polar_hip_fadamw: no host memory to check %llu tensors",
+                  static_cast<unsigned long long>(count));
+    }
   }
   POLAR_HIP_TRY(hipSetDevice(dev->ordinal));
   Table table{};

@@ -41,6 +41,7 @@ constexpr uint32_t kShortList = 64;                       // segments whose logi
 constexpr uint32_t kStagedAt = 12288;                     // bytes in front of the staged packs of a part of one tile
 constexpr uint64_t kMaxCols = 1ull << 24;                 // places are exact as fp32 tokens
 constexpr uint64_t kMostGroups = 1ull << 23;              // of a launch, whose lanes are counted in 32 bits
+constexpr float kLeastScale = 0x1p-64f, kMostScale = 0x1p64f; // far from where scale * log2 e overflows or vanishes
 constexpr float kLog2e = 1.44269504088896340736f;
 constexpr float kLn2 = 0.69314718055994530942f;
 
@@ -334,7 +335,9 @@ __global__ __launch_bounds__(kBlock, 5) void logprobKernel(ForwardArgs a) {
       settle(to);
       reference = to;
       limit = to + 64.0f / c;
-      wide = fabsf(to) > 1e30f; // to * c might overflow: a row masked with the type's lowest value
+      // far from zero `rest` is no small correction any more, and to * c may overflow (a row masked
+      // with the type's lowest value): the difference is taken first, one instruction more per logit
+      wide = fabsf(to) * fmaxf(c, 1.0f) > 0x1p20f;
       shift = wide ? 0.0f : -to * c;
       rest = wide ? 0.0f : __builtin_fmaf(-to, c, -shift);
     }
@@ -704,7 +707,7 @@ int polar_hip_flogprob(polar_hip_device* dev, int type, const void* logits, uint
   POLAR_HIP_REQUIRE(knownType(type), "unknown element type");
   POLAR_HIP_REQUIRE(knownIndex(tokenType), "unknown token type");
   POLAR_HIP_REQUIRE(cols >= 1 && cols <= kMaxCols, "rows of 1 to 2^24 logits");
-  POLAR_HIP_REQUIRE(scale > 0.0f && std::isfinite(scale), "scale must be positive and finite");
+  POLAR_HIP_REQUIRE(scale >= kLeastScale && scale <= kMostScale, "scale must lie between 2^-64 and 2^64");
   POLAR_HIP_REQUIRE(top <= POLAR_HIP_LOGPROB_MAX_TOP && top <= cols, "too many alternatives");
   if (rows == 0) return POLAR_HIP_OK;
   POLAR_HIP_REQUIRE(logits != nullptr, "null tensor");
@@ -736,7 +739,7 @@ int polar_hip_flogprob_grad(polar_hip_device* dev, int type, const void* logits,
   POLAR_HIP_REQUIRE(knownType(type), "unknown element type");
   POLAR_HIP_REQUIRE(knownIndex(tokenType), "unknown token type");
   POLAR_HIP_REQUIRE(cols >= 1 && cols <= kMaxCols, "rows of 1 to 2^24 logits");
-  POLAR_HIP_REQUIRE(scale > 0.0f && std::isfinite(scale), "scale must be positive and finite");
+  POLAR_HIP_REQUIRE(scale >= kLeastScale && scale <= kMostScale, "scale must lie between 2^-64 and 2^64");
   if (rows == 0) return POLAR_HIP_OK;
   POLAR_HIP_REQUIRE(logits && dlogits, "null tensor");
   POLAR_HIP_REQUIRE(dlogprob == nullptr || tokens != nullptr, "log probabilities need tokens");

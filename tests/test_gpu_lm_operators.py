@@ -237,6 +237,8 @@ def check_logprob(dev, x, tokens, kind, scale, top, token_dtype="i64", stride=No
     dev.flogprob(X, T, LP, rows, cols, scale=scale, stats=S, entropy=H, top=top, top_index=TI, top_logprob=TL, dtype=kind,
                  token_dtype=token_dtype, stride=X.stride)
     logsum_tol, lp_tol, entropy_tol = logprob_tolerances(r)
+    with np.errstate(over="ignore"):   # what fp32 does not hold is -infinity
+        r.update({k: r[k].astype(np.float32).astype(np.float64) for k in ("logprob", "top_logprob")})
     stats = S.values()
     assert np.array_equal(stats[:, 0], r["stats"][:, 0])
     close(stats[:, 1], r["stats"][:, 1], logsum_tol, "logsum")
@@ -324,6 +326,17 @@ def test_logprob_of_large_logits_loses_nothing(dev):
     x = ref.rounded(rng.standard_normal((3, 20011)) * 2 + np.array([[1e4], [-3e4], [9e5]]), "f32")
     check_logprob(dev, x, rng.integers(0, 20011, 3), "f32", 1.0, 9)
     check_logprob(dev, x, rng.integers(0, 20011, 3), "f32", 0.9, 2)
+
+
+@pytest.mark.parametrize("scale", [2.0 ** -64, 1e-6, 1e6, 2.0 ** 64])
+def test_logprob_with_extreme_scales(dev, scale):
+    """Almost uniform, and all on the largest: products with the scale may pass what fp32 holds."""
+    _say("flogprob scale", scale)
+    rng = np.random.default_rng(17)
+    x = ref.rounded(rng.standard_normal((4, 9001)) * 3, "f32")
+    x[1] = ref.rounded(rng.standard_normal(9001) * 1e30, "f32")
+    x[2] = ref.rounded(-np.abs(rng.standard_normal(9001)) * 1e12, "f32")
+    check_logprob(dev, x, np.argmax(x, 1), "f32", scale, 4)
 
 
 @pytest.mark.parametrize("cols", [37, 6000, 140001])
@@ -469,6 +482,109 @@ def test_logprob_grad_against_differences_of_the_forward_pass(dev):
         # fp32 results of about ten roundings on values up to 5; the differences are good to 1e-9
         assert abs(got[i] - want) <= 20 * U32 * 5, (i, got[i], want)
     for t in (X, T, LP, H, S, G, DH, D):
+        t.free()
+
+
+@pytest.mark.parametrize("rows", [1, 8, 40])
+def test_logprob_calls_in_a_row_take_nothing_from_each_other(dev, rows):
+    """Rows in parts meet in a workspace that every call uses again: 200 calls on two inputs in turn, some with a product that
+    splits its contraction (the same workspace and counters) between them, each compared with the first of its kind."""
+    _say("flogprob repeated", rows)
+    rng = np.random.default_rng(rows)
+    cols, top = 60011, 11
+    X = [Matrix(dev, "bf16", rows, cols, values=rng.standard_normal((rows, cols))) for _ in range(2)]
+    T = Raw(dev, rng.integers(0, cols, rows).astype(np.int64))
+    outs = [[Raw(dev, np.zeros(rows, np.float32)), Raw(dev, np.zeros(rows, np.float32)), Raw(dev, np.zeros((rows, 2), np.float32)),
+             Raw(dev, np.zeros((rows, top), np.int32)), Raw(dev, np.zeros((rows, top), np.float32))] for _ in range(4)]
+    a, b = dev.array(np.ones(96 * 8192)), dev.array(np.ones(96 * 8192))
+    c = dev.empty(96 * 96)
+
+    def call(i, o):
+        dev.flogprob(X[i], T, o[0], rows, cols, entropy=o[1], stats=o[2], top=top, top_index=o[3], top_logprob=o[4], dtype="bf16")
+    for i in range(2):
+        call(i, outs[i])
+    want = [[t.values() for t in o] for o in outs[:2]]
+    for n in range(100):
+        for i in range(2):
+            call(i, outs[2 + i])
+        if n % 7 == 0:
+            dev.fmatmul(False, True, a, b, c, 96, 96, 8192)
+        if n % 10 == 0:
+            for i in range(2):
+                for t, w in zip(outs[2 + i], want[i]):
+                    assert np.array_equal(t.values(), w)
+    assert np.all(c.download() == 8192)
+    for t in [*X, T, a, b, c, *(t for o in outs for t in o)]:
+        t.free()
+
+
+def test_two_threads_call_one_device(dev):
+    """Calls of two threads on one handle that use its workspace: each thread's results are its own."""
+    _say("two threads")
+    import threading
+    rng = np.random.default_rng(3)
+    rows, cols = 5, 40000
+    jobs = []
+    for i in range(2):
+        x = ref.rounded(rng.standard_normal((rows, cols)), "f32")
+        dy = ref.rounded(rng.standard_normal((64, 300)), "f32")
+        jobs.append(dict(X=Matrix(dev, "f32", rows, cols, values=x), TI=Raw(dev, np.zeros((rows, 6), np.int32)),
+                         TL=Raw(dev, np.zeros((rows, 6), np.float32)), want=ref.logprob(x, np.zeros(rows, int), 1.0, 6)["top_index"],
+                         DY=Matrix(dev, "f32", 64, 300, values=dy), DB=Raw(dev, np.zeros(300, np.float32)), db=dy.sum(0), bad=[]))
+
+    def work(j):
+        for _ in range(60):
+            dev.flogprob(j["X"], None, None, rows, cols, top=6, top_index=j["TI"], top_logprob=j["TL"])
+            dev.flayernorm_grad(j["DY"], j["DY"], None, None, None, j["DB"], 64, 300)
+            if not np.array_equal(j["TI"].values(), j["want"]) or np.abs(j["DB"].values() - j["db"]).max() > 1e-4:
+                j["bad"].append(1)
+    threads = [threading.Thread(target=work, args=(j,)) for j in jobs]
+    for t in threads:
+        t.start()
+    for t in threads:
+        t.join()
+    assert not jobs[0]["bad"] and not jobs[1]["bad"]
+    for j in jobs:
+        for k in ("X", "TI", "TL", "DY", "DB"):
+            j[k].free()
+
+
+def test_rows_whose_offsets_pass_32_bits(dev):
+    """Three rows 2^31 + 5 elements apart (8.6 GB): every row is read and written where it lies."""
+    _say("far rows")
+    rng = np.random.default_rng(9)
+    cols, stride = 5003, (1 << 31) + 5
+    base = dev.alloc_bytes(2 * (2 * stride + cols + 8))
+    x = ref.rounded(rng.standard_normal((3, cols)), "bf16")
+
+    def put(values):
+        for i in range(3):
+            row = ref.store(values[i], "bf16")
+            dev.copy_to_device(base + 2 * i * stride, row.ctypes.data, row.nbytes)
+
+    def get():
+        out = np.empty((3, cols), np.uint16)
+        for i in range(3):
+            dev.copy_to_host(out[i].ctypes.data, base + 2 * i * stride, out[i].nbytes)
+        return ref.widen(out, "bf16")
+    N, T = Matrix(dev, "bf16", 3, cols, values=x), Raw(dev, np.array([1, 2, cols - 1], np.int64))
+    S, G = [Raw(dev, np.zeros((3, 2), np.float32)) for _ in range(2)], Raw(dev, np.ones(3, np.float32))
+    I, P = [Raw(dev, np.zeros((3, 4), np.int32)) for _ in range(2)], Raw(dev, np.zeros((3, 4), np.float32))
+    for at, st, s, i in ((base, stride, S[0], I[0]), (N, cols, S[1], I[1])):
+        put(x)
+        dev.flogprob(at, T, None, 3, cols, stats=s, top=4, top_index=i, top_logprob=P, dtype="bf16", stride=st)
+        dev.flogprob_grad(at, T, s, G, at, 3, cols, dtype="bf16", stride=st, dlogits_stride=st)
+        dev.flayernorm(at, None, None, at, 3, cols, dtype="bf16", x_stride=st, out_stride=st)
+        dev.flayernorm_grad(at, at, None, at, None, None, 3, cols, dtype="bf16", x_stride=st, grad_stride=st, dx_stride=st)
+        if at == base:
+            far = get()
+    N.whole = N._download()   # what was written in place is checked against the far rows, not against the start
+    near = N.values()
+    assert np.array_equal(far, near) and np.isfinite(far).all() and far.any()
+    assert np.array_equal(S[0].values(), S[1].values()) and np.array_equal(I[0].values(), I[1].values())
+    dev._free(base)
+    dev.pool_trim()
+    for t in (N, T, G, P, *S, *I):
         t.free()
 
 
@@ -634,6 +750,29 @@ def test_adamw_keeps_nan_and_infinity_in_their_elements(dev, state):
         # an update is lr in size at most about the first steps: sqrt(v) and m of one gradient; the states' rounding
         # moves it by 1/8 of lr per state
         assert np.abs(got - clean)[~bad].max() <= 0.25e-3
+
+
+def test_adamw_beyond_32_bit_offsets(dev):
+    """A tensor of 2^30 + 1027 fp32 elements (4 GiB a buffer): its last elements are updated like its first."""
+    _say("fadamw 2^30 elements")
+    n = (1 << 30) + 1027
+    bufs = [dev.empty(n) for _ in range(4)]
+    for b, v in zip(bufs, (0.5, 0.25, 0.125, 0.0625)):
+        dev.ffill(v, b)
+    p, g, m, v = bufs
+    dev.fadamw(capi.adamw_tensors([dict(count=n - 1, param=p, grad=g, m=m, v=v, weight_decay=0.5)]), step=3, **ADAMW)
+    new = ref.adamw(0.5, 0.25, 0.125, 0.0625, 0.5, 3, grad_scale=1.0, **ADAMW)
+    for buf, want, old in ((p, new[0], 0.5), (m, new[1], 0.125), (v, new[2], 0.0625)):
+        for at in (0, 1 << 29, n - 1000):
+            part = np.empty(1000, np.float32)
+            dev.copy_to_host(part.ctypes.data, buf.ptr + 4 * at, part.nbytes)
+            if at == n - 1000:
+                assert part[-1] == np.float32(old)     # behind the tensor's end
+                part = part[:-1]
+            assert np.abs(part - want).max() <= 16 * U32 * abs(want)
+    for b in bufs:
+        b.free()
+    dev.pool_trim()
 
 
 # ---- together ---------------------------------------------------------------------

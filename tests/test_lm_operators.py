@@ -68,7 +68,7 @@ def test_layernorm_grad_refuses(lib, handle, change, words):
 @pytest.mark.parametrize("change,words", [
     (dict(dev=0), "dev is null"), (dict(type=3), "element type"), (dict(tokenType=3), "token type"), (dict(cols=0), "rows of 1"),
     (dict(cols=(1 << 24) + 1, stride=1 << 25), "rows of 1"), (dict(scale=0.0), "scale"), (dict(scale=-1.0), "scale"),
-    (dict(scale=float("inf")), "scale"), (dict(scale=float("nan")), "scale"), (dict(top=33, cols=100, stride=100), "alternatives"),
+    (dict(scale=float("inf")), "scale"), (dict(scale=float("nan")), "scale"), (dict(scale=4e19), "scale"), (dict(scale=1e-20), "scale"), (dict(top=33, cols=100, stride=100), "alternatives"),
     (dict(top=9), "alternatives"), (dict(logits=0), "null"), (dict(tokens=0), "tokens"), (dict(topIndex=0), "alternatives"),
     (dict(topLogprob=0), "alternatives"), (dict(stride=7), "stride"), (dict(tokens=A + 4), "misaligned"),
     (dict(logits=A + 2), "misaligned"), (dict(rows=1 << 62), "too large")])
@@ -101,9 +101,16 @@ CONFIG = dict(param_type=0, grad_type=0, state_bits=32, seed=1, step=1, lr=1e-3,
     ({}, dict(weight_decay=float("nan")), "decay"), ({}, dict(m=A + 1), "misaligned"), ({}, dict(param=A + 2), "misaligned")])
 def test_adamw_refuses(lib, handle, config, tensor, words):
     # the second tensor of the list is the wrong one: nothing is launched for the first either
-    tensors = capi.adamw_tensors([TENSOR, {**TENSOR, **tensor}])
+    tensors = capi.adamw_tensors([{**TENSOR, "param": A + 4096}, {**TENSOR, **tensor}])
     c = capi.AdamWConfig(*{**CONFIG, **config}.values())
     refused(lib, lib.polar_hip_fadamw(handle, C.byref(c), tensors, 2), "polar_hip_fadamw", words)
+
+
+def test_adamw_refuses_parameters_that_overlap(lib, handle):
+    c = capi.AdamWConfig(*CONFIG.values())
+    for at in (A, A + 36, A - 36):   # ten elements of four bytes each
+        tensors = capi.adamw_tensors([TENSOR, {**TENSOR, "param": A + 8192}, {**TENSOR, "param": at}])
+        refused(lib, lib.polar_hip_fadamw(handle, C.byref(c), tensors, 3), "overlap")
 
 
 def test_adamw_refuses_null_arguments(lib, handle):
