@@ -100,10 +100,13 @@ __device__ __forceinline__ void rankKeys(const uint64_t* keys, uint32_t count, u
 }
 
 // A lower bound, as an order number, of the `wanted`-th best of the work-group's
-// values: the wanted-th best of its lanes' own best (`order`; 0 for a lane without
-// any), with the bits behind the first kBits cleared.  The first wave finds it bit
-// by bit, counting with ballots the lanes that reach a candidate: compares are its
-// only vector instructions, the rest is scalar.
+// values: the wanted-th best of 64 groups of them (a lane of each wave; `order` is
+// the best a lane has, 0 if it has none), with the bits behind the first kBits
+// cleared.  The first wave finds it bit by bit, counting with a ballot the groups
+// that reach a candidate.  The group maxima of random data let 24 values pass for
+// 20 wanted, 44 for 32; telling all 256 lanes apart would let fewer pass but takes
+// three times the instructions, and a wave that works alone issues one in ten
+// cycles.
 struct BoundScratch {
   uint32_t lanes[kBlock];
   uint32_t bound;
@@ -112,18 +115,13 @@ template <int kBits> __device__ __forceinline__ uint32_t laneBound(uint32_t orde
   lds.lanes[threadIdx.x] = order;
   __syncthreads();
   if (threadIdx.x < 64) {
-    uint32_t mine[kWaves];
+    uint32_t mine = order;
 #pragma unroll
-    for (int w = 0; w < kWaves; ++w) mine[w] = lds.lanes[w * 64 + threadIdx.x];
+    for (int w = 1; w < kWaves; ++w) mine = max(mine, lds.lanes[w * 64 + threadIdx.x]);
     uint32_t bound = 0;
 #pragma unroll 1 // code that runs once per work-group is mostly waited for: short is fast
-    for (int bit = 31; bit >= 32 - kBits; --bit) {
-      const uint32_t candidate = bound | (1u << bit);
-      uint32_t reach = 0;
-#pragma unroll
-      for (int w = 0; w < kWaves; ++w) reach += __popcll(__ballot(mine[w] >= candidate));
-      bound = reach >= wanted ? candidate : bound;
-    }
+    for (uint32_t bit = 0x80000000u; bit != (1u << (31 - kBits)); bit >>= 1)
+      bound = static_cast<uint32_t>(__popcll(__ballot(mine >= (bound | bit)))) >= wanted ? bound | bit : bound;
     if (threadIdx.x == 0) lds.bound = bound;
   }
   __syncthreads();
@@ -207,12 +205,17 @@ template <typename V> __device__ __forceinline__ V takePart(const unsigned char*
   return __hip_atomic_load(reinterpret_cast<const V*>(at), __ATOMIC_RELAXED, __HIP_MEMORY_SCOPE_AGENT);
 }
 
+__device__ __forceinline__ uint64_t partKey(const unsigned char* slots, uint32_t slotBytes, uint32_t top, uint32_t e) {
+  return takePart<uint64_t>(slots + uint64_t(e / top) * slotBytes + kSumsBytes + e % top * sizeof(uint64_t));
+}
+
 // The row's parts joined, in every wave by itself: a lane per part.
 __device__ __forceinline__ RowSums joinSums(const unsigned char* slots, uint32_t slotBytes, uint32_t parts, float c) {
   RowSums r{-__builtin_inff(), 0.0f, 0.0f};
   for (uint32_t p = threadIdx.x % 64; p < parts; p += 64) {
     const unsigned char* at = slots + uint64_t(p) * slotBytes;
-    r = join(r, RowSums{takePart<float>(at), takePart<float>(at + 4), takePart<float>(at + 8)}, c);
+    const RowSums part{takePart<float>(at), takePart<float>(at + 4), takePart<float>(at + 8)};
+    r = p < 64 ? part : join(r, part, c);
   }
   const float m = waveMax(r.m);
   const float d = rebase(r.m, m, c), f = __builtin_amdgcn_exp2f(d);
@@ -222,16 +225,15 @@ __device__ __forceinline__ RowSums joinSums(const unsigned char* slots, uint32_t
 // The `top` best of the parts' keys (0 for none) into `best`: those that reach the
 // bound that the lanes' best ones give, ranked.  Where these are too many (logits
 // that are equal all over the row) stretches of the keys are ranked together with the
-// best so far.  `keys` has room for kJoinKeys.
+// best so far.  `first`: the key of the lane's own number; `keys` has room for kJoinKeys.
 constexpr uint32_t kJoinKeys = kMaxListed;
 template <typename T>
 __device__ __forceinline__ void joinKeys(const unsigned char* slots, uint32_t slotBytes, uint32_t parts, uint32_t top,
-                                         uint64_t* keys, uint64_t* best, BoundScratch& scratch, uint32_t* listed) {
+                                         uint64_t first, uint64_t* keys, uint64_t* best, BoundScratch& scratch,
+                                         uint32_t* listed) {
   const uint32_t all = parts * top;
-  auto keyAt = [&](uint32_t e) {
-    return takePart<uint64_t>(slots + uint64_t(e / top) * slotBytes + kSumsBytes + e % top * sizeof(uint64_t));
-  };
-  uint64_t first = threadIdx.x < all ? keyAt(threadIdx.x) : 0, mine = first;
+  auto keyAt = [&](uint32_t e) { return partKey(slots, slotBytes, top, e); };
+  uint64_t mine = first;
   for (uint32_t e = threadIdx.x + kBlock; e < all; e += kBlock) mine = keyAt(e) > mine ? keyAt(e) : mine;
   if (threadIdx.x == 0) *listed = 0;
   const uint32_t least = laneBound<T::kOrderBits>(static_cast<uint32_t>(mine >> 32), top, scratch);
@@ -433,23 +435,33 @@ __global__ __launch_bounds__(kBlock, 5) void logprobKernel(ForwardArgs a) {
     if (!exact) {
       const uint32_t lowest = orderOf(-__builtin_inff());
       const float low = least <= lowest ? -__builtin_inff() : valueOf(least); // orders below -infinity's are no numbers
-      const uint32_t room = tiles > 1 ? kMaxListed : kStagedAt / sizeof(uint64_t), packs = listed * kPacks;
-      for (uint32_t e = threadIdx.x; e < packs; e += kBlock) {
-        const uint32_t segment = list[e / kPacks];
-        const uint32_t from = place(segment / kBlock, e % kPacks, segment % kBlock);
-        float w[kVec];
-        T::unpack(tiles > 1 ? loadPack<T, false>(x, from, end, kNothing) : staged[e], w);
-        uint32_t n = 0;
-#pragma unroll
-        for (int i = 0; i < kVec; ++i) n += w[i] >= low && from + i < end;
-        if (n == 0) continue;
-        uint32_t at = atomicAdd(&found, n);
-#pragma unroll
-        for (int i = 0; i < kVec; ++i)
-          if (w[i] >= low && from + i < end) {
-            if (at < room) keys[at] = keyOf(w[i], from + i);
-            ++at;
+      const uint32_t room = tiles > 1 ? kMaxListed : kStagedAt / sizeof(uint64_t), segmentsListed = listed;
+      if (tiles == 1) { // an element per lane: short code
+        const Stored* elements = reinterpret_cast<const Stored*>(staged);
+#pragma unroll 1
+        for (uint32_t e = threadIdx.x; e < segmentsListed * kLane; e += kBlock) {
+          const float w = T::widen(elements[e]);
+          const uint32_t at = place(0, e % kLane / kVec, list[e / kLane]) + e % kVec;
+          if (w >= low && at < end) {
+            const uint32_t slot = atomicAdd(&found, 1u);
+            if (slot < room) keys[slot] = keyOf(w, at);
           }
+        }
+      } else { // a pack per lane: one load
+        for (uint32_t e = threadIdx.x; e < segmentsListed * kPacks; e += kBlock) {
+          const uint32_t segment = list[e / kPacks];
+          const uint32_t from = place(segment / kBlock, e % kPacks, segment % kBlock);
+          float w[kVec];
+          T::unpack(loadPack<T, false>(x, from, end, kNothing), w);
+          uint32_t n = 0;
+#pragma unroll
+          for (int i = 0; i < kVec; ++i) n += w[i] >= low && from + i < end;
+          if (n == 0) continue;
+          uint32_t at = atomicAdd(&found, n);
+#pragma unroll
+          for (int i = 0; i < kVec; ++i)
+            if (w[i] >= low && from + i < end) keys[at++] = keyOf(w[i], from + i);
+        }
       }
       __syncthreads();
       exact = found > room;
@@ -559,9 +571,11 @@ __global__ __launch_bounds__(kBlock, 5) void logprobKernel(ForwardArgs a) {
     if (listed == 0) return; // the whole work-group
     if (threadIdx.x == 0) __hip_atomic_store(&a.arrived[rowInLaunch], 0u, __ATOMIC_RELAXED, __HIP_MEMORY_SCOPE_AGENT);
     const unsigned char* slots = a.slots + uint64_t(rowInLaunch) * a.parts * a.slotBytes;
+    uint64_t first = 0; // on its way while the sums are joined
+    if (kTop && threadIdx.x < a.parts * a.top) first = partKey(slots, a.slotBytes, a.top, threadIdx.x);
     total = joinSums(slots, a.slotBytes, a.parts, c);
     if constexpr (kTop)
-      joinKeys<T>(slots, a.slotBytes, a.parts, a.top, reinterpret_cast<uint64_t*>(area), best, scratch, &found);
+      joinKeys<T>(slots, a.slotBytes, a.parts, a.top, first, reinterpret_cast<uint64_t*>(area), best, scratch, &found);
   }
   finishRow(a, row, given, total, best);
 }
