@@ -200,6 +200,30 @@ __global__ __launch_bounds__(kLongBlock) void layerNormLongKernel(
 
 // ---- gradient --------------------------------------------------------------------
 
+// A lane's sums for dw and db of its columns, kept over its team's rows: in registers, or,
+// for teams of sixteen waves, whose lanes have 128 registers, in LDS (a place of its own for
+// each lane and column, the lanes side by side).
+constexpr int kMostRegisterWaves = 8;
+template <int kWaves, int kPacks, int kVec> struct ColumnSums {
+  static constexpr bool kInLds = kWaves > kMostRegisterWaves;
+  static constexpr int kLanes = kWaves * 64;
+  static constexpr uint32_t kLdsBytes = kInLds ? kLanes * kPacks * kVec * sizeof(Float2) : 0;
+  Float2 held[kInLds ? 1 : kPacks * kVec];
+  Float2* lds; // the lane's first place
+
+  __device__ __forceinline__ void clear(Float2* area) {
+    lds = area + threadIdx.x;
+#pragma unroll
+    for (int i = 0; i < kPacks * kVec; ++i) at(i) = Float2{0.0f, 0.0f};
+  }
+  __device__ __forceinline__ Float2& at(int i) {
+    if constexpr (kInLds)
+      return lds[i * kLanes];
+    else
+      return held[i];
+  }
+};
+
 // sums: [2][teams of the whole grid][cols] fp32, dw's before db's; null if neither is wanted
 template <typename T, typename P, int kWaves, int kPacks, int kAhead, bool kStats>
 __global__ __launch_bounds__(kWaves * 64 < kTeamBlock ? kTeamBlock : kWaves * 64) void layerNormGradKernel(
@@ -216,7 +240,10 @@ __global__ __launch_bounds__(kWaves * 64 < kTeamBlock ? kTeamBlock : kWaves * 64
   const uint64_t step = uint64_t(gridDim.x) * kTeams;
   const float count = static_cast<float>(cols);
 
-  float w[kPacks][T::kVec], dw[kPacks][T::kVec], db[kPacks][T::kVec];
+  extern __shared__ Float2 columnArea[];
+  float w[kPacks][T::kVec];
+  ColumnSums<kWaves, kPacks, T::kVec> column;
+  column.clear(columnArea);
   uint64_t row = uint64_t(blockIdx.x) * kTeams + team;
   Pack nextX[kAhead][kPacks], nextDy[kAhead][kPacks];
   float nextMean[kAhead], nextRstd[kAhead];
@@ -233,11 +260,8 @@ __global__ __launch_bounds__(kWaves * 64 < kTeamBlock ? kTeamBlock : kWaves * 64
     if (row + n * step < rows) load(n, row + n * step);
   }
 #pragma unroll
-  for (int k = 0; k < kPacks; ++k) {
+  for (int k = 0; k < kPacks; ++k)
     loadParams<P, T::kVec>(weight, (uint64_t(k) * kLanes + lane) * T::kVec, cols, 1.0f, w[k]);
-#pragma unroll
-    for (int i = 0; i < T::kVec; ++i) dw[k][i] = db[k][i] = 0.0f;
-  }
   int round = 0;
   for (uint64_t first = uint64_t(blockIdx.x) * kTeams; first < rows;) {
 #pragma unroll
@@ -278,8 +302,9 @@ __global__ __launch_bounds__(kWaves * 64 < kTeamBlock ? kTeamBlock : kWaves * 64
           // behind the row's end dy is zero, so that whatever h is there counts for nothing
           h[k][i] = (h[k][i] - mean) * rstd;
           if (here) {
-            dw[k][i] += g[k][i] * h[k][i];
-            db[k][i] += g[k][i];
+            Float2& sum = column.at(k * T::kVec + i);
+            sum.x += g[k][i] * h[k][i];
+            sum.y += g[k][i];
           }
           g[k][i] *= w[k][i];
           s.x += g[k][i];
@@ -306,8 +331,9 @@ __global__ __launch_bounds__(kWaves * 64 < kTeamBlock ? kTeamBlock : kWaves * 64
 #pragma unroll
       for (int i = 0; i < T::kVec; ++i)
         if (c + i < cols) {
-          sums[mine * cols + c + i] = dw[k][i];
-          sums[(teams + mine) * cols + c + i] = db[k][i];
+          const Float2 sum = column.at(k * T::kVec + i);
+          sums[mine * cols + c + i] = sum.x;
+          sums[(teams + mine) * cols + c + i] = sum.y;
         }
     }
   }
@@ -472,6 +498,9 @@ template <typename T, typename P> int norm(polar_hip_device* dev, const NormArgs
   if (wavePacks <= 8) return launchNorm<T, P, 4, 2, 1, 4>(dev, a);
   if (wavePacks <= 16) return launchNorm<T, P, 8, 2, 4, 1>(dev, a);
   if (wavePacks <= 32) return launchNorm<T, P, 16, 2, 1, 1>(dev, a);
+  if constexpr (T::kVec == 4) {
+    if (wavePacks <= 64) return launchNorm<T, P, 16, 4, 1, 1>(dev, a);
+  }
   POLAR_HIP_TRY(launchKernel(dev, layerNormLongKernel<T, P>, dim3(gridFor(a.rows, 1, 1u << 20)), dim3(kLongBlock),
                              static_cast<const typename T::Stored*>(a.x), a.xStride,
                              static_cast<const typename P::Stored*>(a.weight),
@@ -503,11 +532,23 @@ int launchNormGrad(polar_hip_device* dev, const NormGradArgs& a) {
   }
   auto kernel = a.mean == nullptr ? layerNormGradKernel<T, P, kWaves, kPacks, kAhead, true>
                                   : layerNormGradKernel<T, P, kWaves, kPacks, kAhead, false>;
-  POLAR_HIP_TRY(launchKernel(dev, kernel, dim3(grid), dim3(kBlock), static_cast<const typename T::Stored*>(a.dy),
-                             a.dyStride, static_cast<const typename T::Stored*>(a.x), a.xStride,
-                             static_cast<const typename P::Stored*>(a.weight), a.mean, a.rstd, a.eps,
-                             static_cast<typename T::Stored*>(a.dx), a.dxStride, static_cast<float*>(area), a.rows,
-                             static_cast<uint32_t>(a.cols)));
+  constexpr uint32_t ldsBytes = ColumnSums<kWaves, kPacks, T::kVec>::kLdsBytes;
+  if constexpr (ldsBytes > 48 * 1024) { // has to be asked for, once per kernel and device (asking twice is harmless)
+    static std::atomic<uint64_t> raised[2]; // with statistics of its own, and without
+    const uint64_t bit = 1ull << (dev->ordinal & 63);
+    std::atomic<uint64_t>& done = raised[a.mean == nullptr];
+    if (!(done.load(std::memory_order_acquire) & bit)) {
+      POLAR_HIP_TRY(hipFuncSetAttribute(reinterpret_cast<const void*>(kernel), hipFuncAttributeMaxDynamicSharedMemorySize,
+                                        int(ldsBytes)));
+      done.fetch_or(bit, std::memory_order_release);
+    }
+  }
+  POLAR_HIP_TRY(launchKernelLds(dev, kernel, dim3(grid), dim3(kBlock), ldsBytes,
+                                static_cast<const typename T::Stored*>(a.dy), a.dyStride,
+                                static_cast<const typename T::Stored*>(a.x), a.xStride,
+                                static_cast<const typename P::Stored*>(a.weight), a.mean, a.rstd, a.eps,
+                                static_cast<typename T::Stored*>(a.dx), a.dxStride, static_cast<float*>(area), a.rows,
+                                static_cast<uint32_t>(a.cols)));
   return params ? launchParams<P>(dev, a, static_cast<const float*>(area), teams) : POLAR_HIP_OK;
 }
 
@@ -549,7 +590,12 @@ template <typename T, typename P> int normGrad(polar_hip_device* dev, const Norm
   if (wavePacks <= 4) return launchNormGrad<T, P, 4, 1, 2, 2>(dev, a);
   if (wavePacks <= 8) return launchNormGrad<T, P, 8, 1, 4, 1>(dev, a);
   if (wavePacks <= 16) return launchNormGrad<T, P, 8, 2, 2, 1>(dev, a);
-  if (wavePacks <= 32) return launchNormGrad<T, P, 8, 4, 1, 1>(dev, a); // 16 waves would have 128 registers each, and spill
+  if constexpr (T::kVec == 8) {
+    if (wavePacks <= 32) return launchNormGrad<T, P, 16, 2, 1, 1>(dev, a);
+  } else {
+    if (wavePacks <= 32) return launchNormGrad<T, P, 8, 4, 1, 1>(dev, a);
+    if (wavePacks <= 64) return launchNormGrad<T, P, 16, 4, 1, 1>(dev, a);
+  }
   return launchLongGrad<T, P>(dev, a);
 }
 
