@@ -6,7 +6,7 @@
 // Everything is read once and written once: memory is what bounds it.  100
 // million elements in fp32 (28 bytes each) take 457 us, 6.2 TB/s, 91 % of what
 // a large copy reaches; 260 million with states in 8 bits, bf16 gradients and
-// copies (16 bytes each) 708 us, 6.1 TB/s.  Loads and stores stream past the
+// copies (16 bytes each) 705 us, 6.1 TB/s.  Loads and stores stream past the
 // caches (with plain loads or plain stores 510 us).  A launch covers up to
 // kTensors tensors, whose table travels in the kernel's arguments: no table in
 // device memory to upload and keep, and a model of a few hundred tensors takes
@@ -147,9 +147,9 @@ __device__ __forceinline__ uint32_t waveLargest(uint32_t v) {
   return static_cast<uint32_t>(__builtin_amdgcn_readlane(static_cast<int>(v), 63));
 }
 
-// 32 random bits of an element: a multiply-xorshift hash of its number and the
-// seed (two rounds with the odd constants of the 32-bit finaliser of MurmurHash3,
-// published by its author Austin Appleby into the public domain)
+// 32 random bits of an element from its number and the seed: two rounds, each of which
+// folds the word's upper half into its lower one and multiplies by an odd constant, so
+// that every bit of the input reaches every bit of the result
 __device__ __forceinline__ uint32_t randomBits(uint32_t seed, uint64_t element) {
   uint32_t h = static_cast<uint32_t>(element) * 0x9e3779b1u + static_cast<uint32_t>(element >> 32) * 0x85ebca77u + seed;
   h = (h ^ (h >> 16)) * 0x85ebca6bu;

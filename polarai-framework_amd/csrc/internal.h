@@ -80,8 +80,9 @@ struct polar_hip_device {
   // polar_hip_fsoftmax_static works in (resolved once, at open)
   void* softmaxScratch = nullptr;
 
-  // Workspace of the builtins that run more than one kernel per call (softmax
-  // partial sums, split-K partial products): one block that grows on demand to
+  // Workspace of the builtins whose work-groups leave something to a later
+  // kernel or to each other (softmax partial sums, split-K partial products, a
+  // layer norm's column sums, the parts of a row of logits): one block that grows on demand to
   // the largest request seen so far (workspaceFor), so that a call whose size
   // has been seen before neither allocates nor waits.  workspaceMu is held
   // while a call enqueues the kernels that share it.
@@ -89,7 +90,8 @@ struct polar_hip_device {
   void* workspace = nullptr;
   uint64_t workspaceBytes = 0;
   // One arrival counter per C tile of a split contraction whose last-arriving
-  // work-group adds the partial products itself (matmul.hip).  Allocated and
+  // work-group adds the partial products itself (matmul.hip), or per row of logits
+  // in parts (logprob.hip).  Allocated and
   // zeroed when the device is opened; the group that completes a tile sets its
   // counter back to zero, so every launch finds zeros.  Used under workspaceMu.
   uint32_t* tileCounters = nullptr;

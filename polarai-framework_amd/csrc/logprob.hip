@@ -10,7 +10,11 @@
 // only when a logit exceeds it by 2^64 in the exponential: sums in fp32 have
 // the room, and a tile of up to 32 logits per lane costs one comparison instead
 // of a rescaling.  Lanes, waves and parts of a row are joined relative to the
-// true maximum.
+// true maximum.  Memory bounds it, with the vector units close behind (nine issue
+// slots per 16-bit logit, four of them the exponential's): 4096 rows of 131072
+// bf16 160 us without alternatives (6.7 TB/s), 173 with eight; of 65536 fp32 155
+// and 165.  Eight rows of 131072 with twenty alternatives take 10.7 us, one row
+// 9.8: there it is the chain of steps that counts.
 //
 // Alternatives cost next to nothing while the row streams by: a lane notes the
 // maximum of each of its tiles (a "segment") in LDS.  The k-th best of the
@@ -196,7 +200,7 @@ __device__ __forceinline__ void finishRow(const ForwardArgs& a, uint64_t row, Gi
 // best keys) with stores that are visible to the whole device (written through the
 // XCD's L2), is acknowledged, and only then counted.  No fence: writing back and
 // invalidating an L2 per work-group costs far more than all of this (64 rows of
-// 131072 in sixteen parts: 33 us with fences, 15 with a second kernel).
+// 131072 in sixteen parts: 33 us with fences, 15 with a second kernel, 14 so).
 constexpr uint32_t kSumsBytes = 16;
 template <typename V> __device__ __forceinline__ void putPart(unsigned char* at, V value) {
   __hip_atomic_store(reinterpret_cast<V*>(at), value, __ATOMIC_RELAXED, __HIP_MEMORY_SCOPE_AGENT);
@@ -382,7 +386,7 @@ __global__ __launch_bounds__(kBlock, 5) void logprobKernel(ForwardArgs a) {
           asm volatile("" : "+v"(again));
 #pragma unroll
           for (int i = 0; i < kLane; ++i) {
-                const float y = __builtin_fmaf(v[i], again, shift);
+            const float y = __builtin_fmaf(v[i], again, shift);
             t1 = __builtin_fmaf(__builtin_amdgcn_exp2f(y), fmaxf(y, -160.0f), t1);
           }
         }
@@ -646,7 +650,7 @@ __global__ __launch_bounds__(kGradBlock) void logprobGradKernel(GradArgs a) {
 template <typename T> int forward(polar_hip_device* dev, ForwardArgs a, uint64_t rows, uint64_t reserved = 0) {
   const uint32_t tiles = (a.cols + tileCols<T>() - 1) / tileCols<T>();
   // parts: at most kMaxTiles tiles each, and enough of them for two work-groups per CU (64 rows of 131072
-  // bf16 with 20 alternatives: 15.0 us; four per CU 17.8; 512 rows 30.7, 31.4, eight 38.7)
+  // bf16 with 20 alternatives: 14 us, with four per CU 17; 512 rows 31, with eight 39)
   const uint64_t groups = 2ull * dev->info.compute_units;
   const uint64_t wanted = std::max<uint64_t>((tiles + kMaxTiles - 1) / kMaxTiles, groups / std::max<uint64_t>(rows, 1));
   a.tilesPerPart = static_cast<uint32_t>((tiles + std::min<uint64_t>(wanted, tiles) - 1) / std::min<uint64_t>(wanted, tiles));

@@ -195,3 +195,15 @@ def test_token_head_graphs_call_sequence_on_the_mock_device():
             h.run()
             h.clear_program()
         assert h.counters().launches == 3 + 5 + 4
+
+
+def test_operands_are_buffers_tensors_of_other_libraries_or_addresses():
+    class Foreign:
+        def data_ptr(self):
+            return 4096
+
+    class Own:
+        ptr = 8192
+    plan = capi.adamw_tensors([dict(count=3, param=Foreign(), grad=Own(), m=12288, v=None, weight_decay=0.25, first=1 << 40)])
+    assert (plan[0].param, plan[0].grad, plan[0].m, plan[0].v) == (4096, 8192, 12288, None)
+    assert (plan[0].count, plan[0].first, plan[0].weight_decay, plan[0].master) == (3, 1 << 40, 0.25, None)
