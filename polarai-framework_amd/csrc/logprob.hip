@@ -200,7 +200,11 @@ __device__ __forceinline__ void finishRow(const ForwardArgs& a, uint64_t row, Gi
 // best keys) with stores that are visible to the whole device (written through the
 // XCD's L2), is acknowledged, and only then counted.  No fence: writing back and
 // invalidating an L2 per work-group costs far more than all of this (64 rows of
-// 131072 in sixteen parts: 33 us with fences, 15 with a second kernel, 14 so).
+// 131072 in sixteen parts, when it was taken: 33 us with fences, 18 so).  A second
+// kernel for the join was faster there (15) and slower for eight rows (15, against
+// 13.5 so), which is the call that waits on every token; the one launch was kept
+// for those.  Since then 64 rows take eight parts, 14.0 us, and would take 16.4 in
+// sixteen; a second kernel was not measured again.
 constexpr uint32_t kSumsBytes = 16;
 template <typename V> __device__ __forceinline__ void putPart(unsigned char* at, V value) {
   __hip_atomic_store(reinterpret_cast<V*>(at), value, __ATOMIC_RELAXED, __HIP_MEMORY_SCOPE_AGENT);
@@ -650,7 +654,8 @@ __global__ __launch_bounds__(kGradBlock) void logprobGradKernel(GradArgs a) {
 template <typename T> int forward(polar_hip_device* dev, ForwardArgs a, uint64_t rows, uint64_t reserved = 0) {
   const uint32_t tiles = (a.cols + tileCols<T>() - 1) / tileCols<T>();
   // parts: at most kMaxTiles tiles each, and enough of them for two work-groups per CU (64 rows of 131072
-  // bf16 with 20 alternatives: 14 us, with four per CU 17; 512 rows 31, with eight 39)
+  // bf16 with 20 alternatives: 14.0 us, with four per CU 16.4; 512 rows 28.5, 32 and with eight 40; eight rows
+  // have a part per tile, 11, whichever it is)
   const uint64_t groups = 2ull * dev->info.compute_units;
   const uint64_t wanted = std::max<uint64_t>((tiles + kMaxTiles - 1) / kMaxTiles, groups / std::max<uint64_t>(rows, 1));
   a.tilesPerPart = static_cast<uint32_t>((tiles + std::min<uint64_t>(wanted, tiles) - 1) / std::min<uint64_t>(wanted, tiles));
