@@ -4,7 +4,7 @@
 //   p = p - lr wd p - (lr / (1 - b1^t)) m / (sqrt(v) / sqrt(1 - b2^t) + eps)
 //
 // Everything is read once and written once: memory is what bounds it.  100
-// million elements in fp32 (28 bytes each) take 457 us, 6.2 TB/s, 91 % of what
+// million elements in fp32 (28 bytes each) take 457 us, 6.2 TB/s, 90 % of what
 // a large copy reaches; 260 million with states in 8 bits, bf16 gradients and
 // copies (16 bytes each) 705 us, 6.1 TB/s.  Loads and stores stream past the
 // caches (with plain loads or plain stores 510 us).  A launch covers up to
@@ -147,11 +147,13 @@ __device__ __forceinline__ uint32_t waveLargest(uint32_t v) {
   return static_cast<uint32_t>(__builtin_amdgcn_readlane(static_cast<int>(v), 63));
 }
 
-// 32 random bits of an element from its number and the seed: two rounds, each of which
-// folds the word's upper half into its lower one and multiplies by an odd constant, so
-// that every bit of the input reaches every bit of the result
+// 32 random bits of an element.  Its number and the seed become one word (the number's
+// lower half times 2^32 over the golden ratio, rounded to a prime; the upper half times
+// the fraction of the root of two in 32 bits), which goes through a published mix: the
+// shifts and the two constants are those of MurmurHash3's 32-bit finaliser (Austin
+// Appleby, public domain).
 __device__ __forceinline__ uint32_t randomBits(uint32_t seed, uint64_t element) {
-  uint32_t h = static_cast<uint32_t>(element) * 0x9e3779b1u + static_cast<uint32_t>(element >> 32) * 0x85ebca77u + seed;
+  uint32_t h = static_cast<uint32_t>(element) * 0x9e3779b1u + static_cast<uint32_t>(element >> 32) * 0x6a09e667u + seed;
   h = (h ^ (h >> 16)) * 0x85ebca6bu;
   h = (h ^ (h >> 13)) * 0xc2b2ae35u;
   return h ^ (h >> 16);

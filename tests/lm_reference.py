@@ -155,7 +155,7 @@ E4M3[[0x7F, 0xFF]] = np.nan
 def random_bits(seed, elements):
     e = np.asarray(elements, dtype=np.uint64)
     m = np.uint64(0xFFFFFFFF)
-    h = ((e & m) * np.uint64(0x9E3779B1) + (e >> np.uint64(32)) * np.uint64(0x85EBCA77) + np.uint64(seed)) & m
+    h = ((e & m) * np.uint64(0x9E3779B1) + (e >> np.uint64(32)) * np.uint64(0x6A09E667) + np.uint64(seed)) & m
     h = ((h ^ (h >> np.uint64(16))) * np.uint64(0x85EBCA6B)) & m
     h = ((h ^ (h >> np.uint64(13))) * np.uint64(0xC2B2AE35)) & m
     return h ^ (h >> np.uint64(16))
