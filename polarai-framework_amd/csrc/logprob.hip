@@ -58,8 +58,10 @@ struct RowSums {
 };
 
 // What a sum relative to `from` is multiplied by to be relative to `to` >= from,
-// as an exponent; an empty sum's `from` is -infinity, and both may be.
-__device__ __forceinline__ float rebase(float from, float to, float c) { return fmaxf((from - to) * c, -1e30f); }
+// as an exponent; an empty sum's `from` is -infinity, and both may be.  No less than
+// -300: sums are below 2^80, so that nothing of them is left there, and a sum times the
+// exponent (which s1 needs) stays far from fp32's limit.
+__device__ __forceinline__ float rebase(float from, float to, float c) { return fmaxf((from - to) * c, -300.0f); }
 
 __device__ __forceinline__ RowSums join(RowSums a, RowSums b, float c) {
   const float m = fmaxf(a.m, b.m);

@@ -1,0 +1,64 @@
+"""Layer norm, token log probabilities and AdamW at the ends of what they take: rows whose logits rise by powers of ten,
+norms of constant rows far from zero, several rows per team of waves, 8-bit states of elements that are small in their block.
+Against plain implementations in 64 bits, with the tolerances of test_gpu_lm_operators."""
+import numpy as np
+import pytest
+
+import lm_reference as ref
+from lm_reference import U32, Matrix, Raw
+from test_gpu_lm_operators import close, logprob_tolerances
+
+pytestmark = pytest.mark.gpu
+
+
+def _say(*a):
+    print(*a, flush=True)
+
+
+# ---- log probabilities ------------------------------------------------------------
+
+TILE = {"f32": 4096, "f16": 8192, "bf16": 8192}   # logits that a work-group takes at a time
+LARGEST = {"f32": float(np.finfo(np.float32).max), "f16": 65504.0, "bf16": float(ref.widen(np.array([0x7F7F], np.uint16), "bf16")[0])}
+
+
+def check_repeated_rows(dev, patterns, rows, kind, scale):
+    """Rows that repeat a few patterns, so that there are many of them (which sets how a row is cut into parts) and few to
+    compute in 64 bits."""
+    n, cols = patterns.shape
+    which = np.arange(rows) % n
+    tokens = np.argmax(patterns, 1)
+    r = ref.logprob(patterns, tokens, scale)
+    X, T = Matrix(dev, kind, rows, cols, cols + 1, 1, patterns[which]), Raw(dev, tokens[which].astype(np.int64))
+    LP, H, S = Raw(dev, np.full(rows, 9, np.float32)), Raw(dev, np.full(rows, 9, np.float32)), Raw(dev, np.full((rows, 2), 9, np.float32))
+    dev.flogprob(X, T, LP, rows, cols, scale=scale, stats=S, entropy=H, dtype=kind, stride=X.stride)
+    logsum_tol, lp_tol, entropy_tol = logprob_tolerances(r)
+    stats = S.values()
+    assert np.array_equal(stats[:, 0], r["stats"][which, 0])
+    close(stats[:, 1], r["stats"][which, 1], logsum_tol[which], "logsum")
+    close(H.values(), r["entropy"][which], entropy_tol[which], "entropy")
+    close(LP.values(), r["logprob"][which], lp_tol[np.arange(n), tokens][which], "logprob")
+    for t in (X, T, LP, H, S):
+        t.free()
+
+
+@pytest.mark.parametrize("kind", ["f32", "f16", "bf16"])
+@pytest.mark.parametrize("rows,tiles", [(520, 3), (64, 24), (3, 5)])
+def test_logprob_of_rows_that_rise_before_one_large_logit(dev, kind, rows, tiles):
+    """A wave that has summed terms far above its reference when one very large logit (a forced token) makes all of them
+    nothing: the entropy is that of the large one alone, 0."""
+    _say("flogprob rise", kind, rows, tiles)
+    tile = TILE[kind]
+    cols = tiles * tile - 5
+    step = np.arange(cols) // tile % 3
+    top = min(1e30, LARGEST[kind] / 2)
+
+    def row(first, then, last, at):
+        x = np.where(step == 0, first, then).astype(np.float64)
+        if last is not None:
+            x[at] = last
+        return x
+    end = 2 * tile + 100
+    patterns = np.stack([row(0.0, 20.0, top, end), row(5.0, 25.0, LARGEST[kind], end), row(0.0, 40.0, min(1e20, top), cols - 1),
+                         row(0.0, 20.0, 70.0, end), row(0.0, 20.0, None, 0), row(-30.0, 10.0, top, 3), row(-np.inf, 40.0, top, end),
+                         row(-LARGEST[kind], 20.0, 1000.0, end)])
+    check_repeated_rows(dev, ref.rounded(patterns, kind), rows, kind, 1.0)
