@@ -7,10 +7,10 @@
 //
 // The forward pass reads the logits once.  A wave keeps one reference for its
 // exponentials, the largest logit seen when it was last set, and sets it anew
-// only when a logit exceeds it by 2^64 in the exponential: sums in fp32 have
-// the room, and a tile of up to 32 logits per lane costs one comparison instead
-// of a rescaling.  Lanes, waves and parts of a row are joined relative to the
-// true maximum.  Memory bounds it, with the vector units close behind (nine issue
+// only when a logit exceeds it by 2^64 in the exponential (far from zero, whenever one
+// exceeds it): sums in fp32 have the room, and a tile of up to 32 logits per lane costs
+// one comparison instead of a rescaling.  Lanes, waves and parts of a row are joined
+// relative to the true maximum.  Memory bounds it, with the vector units close behind (nine issue
 // slots per 16-bit logit, four of them the exponential's): 4096 rows of 131072
 // bf16 160 us without alternatives (6.7 TB/s), 173 with eight; of 65536 fp32 155
 // and 165.  Eight rows of 131072 with twenty alternatives take 10.7 us, one row
@@ -346,10 +346,12 @@ __global__ __launch_bounds__(kBlock, 5) void logprobKernel(ForwardArgs a) {
       const float to = waveMax(laneBest);
       settle(to);
       reference = to;
-      limit = to + 64.0f / c;
       // far from zero `rest` is no small correction any more, and to * c may overflow (a row masked
       // with the type's lowest value): the difference is taken first, one instruction more per logit
       wide = fabsf(to) * fmaxf(c, 1.0f) > 0x1p20f;
+      // there the next float above `to` may lie as far as 2^64 is: `to + 64 / c` would be rounded up
+      // to it, and terms of up to 2^128 pass
+      limit = wide ? to : to + 64.0f / c;
       shift = wide ? 0.0f : -to * c;
       rest = wide ? 0.0f : __builtin_fmaf(-to, c, -shift);
     }

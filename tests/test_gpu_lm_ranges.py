@@ -62,3 +62,18 @@ def test_logprob_of_rows_that_rise_before_one_large_logit(dev, kind, rows, tiles
                          row(0.0, 20.0, 70.0, end), row(0.0, 20.0, None, 0), row(-30.0, 10.0, top, 3), row(-np.inf, 40.0, top, end),
                          row(-LARGEST[kind], 20.0, 1000.0, end)])
     check_repeated_rows(dev, ref.rounded(patterns, kind), rows, kind, 1.0)
+
+
+@pytest.mark.parametrize("scale", [1.0, 1.3, 1.38, 2.0 ** 20])
+def test_logprob_of_large_logits_one_step_apart(dev, scale):
+    """Logits so large that neighbours of fp32 lie up to 88 apart in the exponential: terms relative to the smaller one would
+    be up to 2^128 each."""
+    _say("flogprob neighbours", scale)
+    rows, tile = 520, TILE["f32"]
+    patterns = []
+    for size in (6e8, -6e8, 6e8 / 2.0 ** 20, 1.2e9, 3e5):
+        low = np.float32(size)
+        high = np.nextafter(low, np.float32(np.inf))
+        patterns.append(np.where(np.arange(3 * tile) < tile, float(low), float(high)))
+        patterns.append(np.where(np.arange(3 * tile) < 2 * tile, float(low), float(high)))
+    check_repeated_rows(dev, np.stack(patterns), rows, "f32", scale)
