@@ -77,3 +77,39 @@ def test_logprob_of_large_logits_one_step_apart(dev, scale):
         patterns.append(np.where(np.arange(3 * tile) < tile, float(low), float(high)))
         patterns.append(np.where(np.arange(3 * tile) < 2 * tile, float(low), float(high)))
     check_repeated_rows(dev, np.stack(patterns), rows, "f32", scale)
+
+
+# ---- layer norm -------------------------------------------------------------------
+
+
+@pytest.mark.parametrize("kind", ["f32", "bf16"])
+@pytest.mark.parametrize("cols", [1, 5, 127, 515, 1021, 2500, 5000, 8191, 9001, 33001])
+@pytest.mark.parametrize("given", [True, False])
+def test_layernorm_grad_of_constant_rows_far_from_zero(dev, kind, cols, given):
+    """A constant row has h = 0 everywhere, however large its value: what stands behind the row's end takes no part."""
+    _say("flayernorm_grad constant rows", kind, cols, given)
+    rng = np.random.default_rng(cols)
+    x = ref.rounded(rng.standard_normal((4, cols)), kind)
+    # a power of two, whose sum over the row and mean are exact where the statistics are computed again; the reciprocal root
+    # of eps is 316, so that 2^121 times it passes what fp32 holds
+    x[1] = 2.0 ** 121 if given or cols < 100 else 2.0 ** 112
+    x[2] = -2.0 ** 120 if given or cols < 100 else -2.0 ** 111
+    eps = 1e-5 if given or cols < 100 else 1e-20
+    dy = ref.rounded(rng.standard_normal((4, cols)), kind)
+    W = Raw(dev, np.ones(cols, np.float32))
+    mean, rstd = x.mean(1), 1 / np.sqrt(x.var(1) + eps)
+    DY, X, DX = Matrix(dev, kind, 4, cols, values=dy), Matrix(dev, kind, 4, cols, values=x), Matrix(dev, kind, 4, cols)
+    M, R = Raw(dev, mean.astype(np.float32)), Raw(dev, rstd.astype(np.float32))
+    DB = Raw(dev, np.zeros(cols, np.float32))
+    dev.flayernorm_grad(DY, X, W, DX, None, DB, 4, cols, eps=eps, mean=M if given else None, rstd=R if given else None, dtype=kind)
+    got = DX.values()
+    for r in (1, 2):
+        want = rstd[r] * (dy[r] - dy[r].mean())   # h is 0
+        # h is exactly 0 where the mean is exact: it is for rows up to 2^24 elements of one power of two (sums of at most
+        # 24 bits of it); the sum along the row as in check_norm_grad, rstd rounded or computed again (8 u)
+        tol = rstd[r] * (4 * U32 * (np.abs(dy[r]) + np.abs(dy[r]).mean()) + 64 * U32 * np.abs(dy[r]).mean()) + 10 * U32 * np.abs(want)
+        close(got[r], want, tol * 1.01 + ref.HALF_STEP[kind] * np.abs(want) + ref.TINY[kind], f"dx of row {r}")
+    assert np.isfinite(got).all()
+    close(DB.values(), dy.sum(0), 8 * U32 * np.abs(dy).sum(0), "dbias")
+    for t in (W, DY, X, DX, M, R, DB):
+        t.free()
