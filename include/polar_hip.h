@@ -401,7 +401,8 @@ typedef struct polar_hip_adamw_tensor {
   const void* grad;   /* count elements of grad_type                              */
   void* m;            /* first moment: fp32, or 8-bit floats (sign, 4 exponent and */
                       /* 3 mantissa bits, largest 448) that m_scale multiplies     */
-  void* v;            /* second moment: fp32, or its square root as such floats    */
+  void* v;            /* second moment: fp32, or its square root as such floats,   */
+                      /* 0x80 (minus zero): less than the smallest, but not zero   */
   float* master;      /* param_type fp32: not used.  Otherwise the parameters in   */
                       /* fp32, of which param gets a rounded copy                  */
   float* m_scale;     /* 8-bit states: one per 256 elements; else not used         */
@@ -427,8 +428,10 @@ typedef struct polar_hip_adamw_config {
  * anything is launched.  Tensors must not overlap (parameters that do are
  * refused: weights that two layers share are listed once).  8-bit states are rounded
  * stochastically, up where the upper (v) or lower (m) 16 bits of a hash of seed
- * and element number say so; a block whose scale is not above 2^-100 holds zeros,
- * and a state that is not finite is held as NaN, without a say in its block's
+ * and element number say so; a block whose scale is not above 2^-100 holds zeros.
+ * A root that is held as zero without being zero is held as 0x80, and the next
+ * step divides by the smallest float (2^-9) times its scale at least.  A state that
+ * is not finite is held as NaN, without a say in its block's
  * scale. */
 int polar_hip_fadamw(polar_hip_device* dev, const polar_hip_adamw_config* config,
                      const polar_hip_adamw_tensor* tensors, uint64_t count);

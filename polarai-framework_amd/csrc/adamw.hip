@@ -23,6 +23,16 @@
 // of two neighbours (3 to 6 %); stochastically it follows on average.  The 16
 // random bits come from a hash of the caller's seed and the element's number.
 // The parameter is updated from the unrounded states.
+//
+// Below the smallest code (4.4e-6 of the block's largest) a root is held as zero
+// most of the time, and m, whose random bits are others, now and then as a whole
+// code: their quotient was a step of hundreds of lr.  A root that is not zero and
+// rounds to zero therefore leaves a trace, code 0x80 (minus zero: it still counts
+// as 0 for the next root, so that the average is kept), and the next step divides
+// by the smallest code at least: too small a step, as with a larger eps, in place
+// of one that is too large (elements 10^6 times below the largest of their block
+// over 1500 steps: root mean square 0.15 lr and at most 1.5 lr, with states in 32
+// bits 0.23 and 1.1, without the trace 8.3 and 399).
 #include "typed.h"
 
 #include <algorithm>
@@ -132,6 +142,8 @@ __device__ __forceinline__ uint32_t narrowCode(float t, uint32_t random) {
   return code | ((bits >> 24) & 0x80u);
 }
 constexpr uint32_t kNotANumber = 0x7f; // as an 8-bit float
+constexpr uint32_t kTrace = 0x80;      // of a root that is less than the smallest code, but not zero
+constexpr float kSmallest = 0x1p-9f;   // code
 constexpr uint32_t kInfinity = 0x7f800000u;
 
 // Largest of the wave's sizes, given as the bits of fp32 numbers that are not negative:
@@ -175,6 +187,8 @@ __device__ __forceinline__ float rootOf(float v) {
 // parameter's type; one of 16 bits is a copy of the fp32 master.  G: the gradient's.
 template <typename P, typename G, bool kSmall> struct Four {
   float p[4], g[4], m[4], v[4], r[4];
+  uint32_t traces; // of the roots, at their codes' places
+  float leastRoot; // what such a root is at most
 
   __device__ __forceinline__ void load(const Entry& e, const float* master, uint64_t at, int n) {
     load4<TypeF32>(master + at, n, p);
@@ -183,7 +197,10 @@ template <typename P, typename G, bool kSmall> struct Four {
       const uint64_t block = at / kScaleBlock;
       const float ms = e.mScale[block], vs = e.vScale[block];
       widenCodes(loadCodes(static_cast<const uint8_t*>(e.m) + at, n), m);
-      widenCodes(loadCodes(static_cast<const uint8_t*>(e.v) + at, n), r);
+      const uint32_t roots = loadCodes(static_cast<const uint8_t*>(e.v) + at, n);
+      widenCodes(roots, r);
+      traces = roots & (kTrace * 0x01010101u);
+      leastRoot = kSmallest * vs;
 #pragma unroll
       for (int i = 0; i < 4; ++i) {
         m[i] *= ms;
@@ -197,23 +214,36 @@ template <typename P, typename G, bool kSmall> struct Four {
   }
 
   __device__ __forceinline__ void step(const Table& t, float decay) {
-#pragma unroll
-    for (int i = 0; i < 4; ++i) {
+    auto states = [&](int i) {
       g[i] *= t.gradScale;
       m[i] = m[i] * t.beta1 + g[i] * t.rest1;
       v[i] = v[i] * t.beta2 + (g[i] * g[i]) * t.rest2;
-      const float scaled = m[i] * t.stepSize;
-      if constexpr (kSmall) {
-        // The quotient only moves the parameter, by a thousandth or so of its size: the hardware's
-        // reciprocal, good to a unit in the last place, is nothing against the three bits that the
-        // states have.  (The divisor is 0, or far above the subnormal numbers: a root's smallest
-        // value is 3.7e-23.)  With the exact division and sqrtf their 20 instructions more per
-        // element would set the time: 788 us for 260 million elements.
-        r[i] = rootOf(v[i]);
-        p[i] = (p[i] - p[i] * decay) - scaled * __builtin_amdgcn_rcpf(r[i] * t.byCorrection + t.eps);
-      } else {
-        r[i] = sqrtf(v[i]);
-        p[i] = (p[i] - p[i] * decay) - scaled / (r[i] * t.byCorrection + t.eps);
+    };
+    if constexpr (kSmall) {
+      float divisor[4];
+#pragma unroll
+      for (int i = 0; i < 4; ++i) {
+        states(i);
+        divisor[i] = r[i] = rootOf(v[i]);
+      }
+      if (traces != 0) { // rare
+#pragma unroll
+        for (int i = 0; i < 4; ++i)
+          if (traces & (kTrace << (8 * i))) divisor[i] = r[i] < leastRoot ? leastRoot : r[i];
+      }
+      // The quotient only moves the parameter, by a thousandth or so of its size: the hardware's
+      // reciprocal, good to a unit in the last place, is nothing against the three bits that the
+      // states have.  (The divisor is 0, or far above the subnormal numbers: a root's smallest
+      // value is 3.7e-23.)  With the exact division and sqrtf their 20 instructions more per
+      // element would set the time: 788 us for 260 million elements.
+#pragma unroll
+      for (int i = 0; i < 4; ++i)
+        p[i] = (p[i] - p[i] * decay) - m[i] * t.stepSize * __builtin_amdgcn_rcpf(divisor[i] * t.byCorrection + t.eps);
+    } else {
+#pragma unroll
+      for (int i = 0; i < 4; ++i) {
+        states(i);
+        p[i] = (p[i] - p[i] * decay) - m[i] * t.stepSize / (sqrtf(v[i]) * t.byCorrection + t.eps);
       }
     }
   }
@@ -258,6 +288,13 @@ template <typename P, typename G, bool kSmall> struct Four {
           if (!(fabsf(m[i]) < __builtin_inff())) codeM = (codeM & ~(0xffu << (8 * i))) | kNotANumber << (8 * i);
           if (!(fabsf(r[i]) < __builtin_inff())) codeV = (codeV & ~(0xffu << (8 * i))) | kNotANumber << (8 * i);
         }
+      }
+      // codes are below 0x80, so that the sum's upper bit in each byte says whether its code is not 0
+      const uint32_t zeros = ~(codeV + 0x7f7f7f7fu) & 0x80808080u;
+      if (zeros != 0) { // rare, but for elements that never had a gradient
+#pragma unroll
+        for (int i = 0; i < 4; ++i)
+          if (r[i] > 0.0f || m[i] != 0.0f) codeV |= zeros & (kTrace << (8 * i));
       }
       storeCodes(static_cast<uint8_t*>(e.m) + at, n, codeM);
       storeCodes(static_cast<uint8_t*>(e.v) + at, n, codeV);

@@ -6,6 +6,7 @@ import pytest
 
 import lm_reference as ref
 from lm_reference import U32, Matrix, Raw
+from polarai_framework_amd import capi
 from test_gpu_lm_operators import close, logprob_tolerances
 
 pytestmark = pytest.mark.gpu
@@ -112,4 +113,73 @@ def test_layernorm_grad_of_constant_rows_far_from_zero(dev, kind, cols, given):
     assert np.isfinite(got).all()
     close(DB.values(), dy.sum(0), 8 * U32 * np.abs(dy).sum(0), "dbias")
     for t in (W, DY, X, DX, M, R, DB):
+        t.free()
+
+
+# ---- AdamW ------------------------------------------------------------------------
+
+def test_adamw_8_bit_states_with_seven_decades_in_a_block(dev):
+    """Elements whose gradients are 10 to 10 million times smaller than the largest of their block, down to where neither state
+    has a code of its own: their steps stay of the size that AdamW's steps have, a few lr.  What bounds them: |m| / sqrt(v) of
+    the unrounded states is about 1 for such gradients (with the corrections 1.1 at most over these steps); a state near the
+    smallest code is off by a factor of two at most, m up and the root down, so 4.4; and where the root is below the smallest
+    code, m may be a whole code too much, over a divisor of a code: the ratio of the block's two scales, at most 1.1 of its
+    corrections.  6 covers the sum."""
+    _say("fadamw decades")
+    n, steps, lr = 8 * 256, 400, 1e-3
+    rng = np.random.default_rng(31)
+    decade = np.arange(n) % 8
+    decade[(decade == 0) & (np.arange(n) % 256 != 0)] = 1   # the largest is alone in its block
+    P, G = Raw(dev, np.zeros(n, np.float32)), Raw(dev, np.zeros(n, np.float32))
+    M, V = Raw(dev, np.zeros(n, np.uint8)), Raw(dev, np.zeros(n, np.uint8))
+    MS, VS = Raw(dev, np.zeros(n // 256, np.float32)), Raw(dev, np.zeros(n // 256, np.float32))
+    plan = capi.adamw_tensors([dict(count=n, param=P, grad=G, m=M, v=V, m_scale=MS, v_scale=VS)])
+    before, moved = np.zeros(n), []
+    for step in range(1, steps + 1):
+        g = (rng.standard_normal(n) * 10.0 ** -decade).astype(np.float32)
+        dev.copy_to_device(G.ptr, g.ctypes.data, g.nbytes)
+        dev.fadamw(plan, step=step, lr=lr, seed=step, state_dtype="8bit")
+        after = P.values().astype(np.float64)
+        moved.append((after - before) / lr)
+        before = after
+    moved = np.array(moved)
+    largest = np.abs(moved[10:]).max(0)
+    rms = [np.sqrt((moved[10:, decade == d] ** 2).mean()) for d in range(8)]
+    for d in range(8):
+        _say(f"size 1e-{d}: root mean square {rms[d]:.3f} lr, largest {largest[decade == d].max():.2f} lr")
+    assert largest.max() <= 6, largest.max()
+    # what has codes of its own moves as with states in 32 bits
+    assert all(0.15 < rms[d] < 0.35 for d in (1, 2, 3, 4))
+    for t in (P, G, M, V, MS, VS):
+        t.free()
+
+
+def test_adamw_8_bit_roots_below_the_smallest_code(dev):
+    """A root that is not zero and rounds to zero leaves its trace: code 0x80, which stands for 0 too; the next step divides by
+    the smallest code at least.  A root that is zero leaves code 0."""
+    _say("fadamw traces")
+    n = 256
+    g = np.zeros(n, np.float32)
+    g[0], g[1:100], g[100:200] = 1.0, 1e-9, 1e-3
+    P, G = Raw(dev, np.zeros(n, np.float32)), Raw(dev, g)
+    M, V, MS, VS = Raw(dev, np.zeros(n, np.uint8)), Raw(dev, np.zeros(n, np.uint8)), Raw(dev, np.zeros(1, np.float32)), Raw(dev, np.zeros(1, np.float32))
+    plan = capi.adamw_tensors([dict(count=n, param=P, grad=G, m=M, v=V, m_scale=MS, v_scale=VS)])
+    dev.fadamw(plan, step=1, lr=1e-3, seed=5, state_dtype="8bit")
+    codes = V.values()
+    assert (codes[1:100] == 0x80).all() and (codes[200:] == 0).all()
+    assert (codes[100:200] > 0).all() and (codes[100:200] < 0x80).all() and codes[0] == 0x7E
+    # the states of the 2nd step as given: m one code, the root's trace; gradient 0
+    m = np.full(n, 1, np.uint8)
+    dev.copy_to_device(M.ptr, m.ctypes.data, n)
+    before = P.values().astype(np.float64)
+    zero = np.zeros(n, np.float32)
+    dev.copy_to_device(G.ptr, zero.ctypes.data, zero.nbytes)
+    ms, vs = float(MS.values()[0]), float(VS.values()[0])
+    dev.fadamw(plan, step=2, lr=1e-3, seed=6, state_dtype="8bit", eps=0.0)
+    step = before - P.values()
+    m2 = 0.9 * 2.0 ** -9 * ms / (1 - 0.9 ** 2)
+    want = 1e-3 * m2 / (2.0 ** -9 * vs / np.sqrt(1 - 0.999 ** 2))
+    # about ten roundings and a reciprocal good to 2 u, the difference of parameters of 1e-3
+    assert np.abs(step[1:100] - want).max() <= 20 * U32 * want + 4 * U32 * np.abs(before[1:100]).max()
+    for t in (P, G, M, V, MS, VS):
         t.free()
