@@ -425,14 +425,14 @@ typedef struct polar_hip_adamw_config {
  *   param = param - lr weight_decay param
  *           - lr / (1 - beta1^step) m / (sqrt(v) / sqrt(1 - beta2^step) + eps)
  * The list is read before the call returns.  All of it is checked before
- * anything is launched.  Tensors must not overlap (parameters that do are
- * refused: weights that two layers share are listed once).  8-bit states are rounded
- * stochastically, up where the upper (v) or lower (m) 16 bits of a hash of seed
- * and element number say so; a block whose scale is not above 2^-100 holds zeros.
- * A root that is held as zero without being zero is held as 0x80, and the next
- * step divides by the smallest float (2^-9) times its scale at least.  A state that
- * is not finite is held as NaN, without a say in its block's
- * scale. */
+ * anything is launched.  Buffers that are written must not overlap and are
+ * refused if they do (weights that two layers share are listed once), nor may a
+ * gradient overlap one of them.  8-bit states are rounded stochastically, up where
+ * the upper (v) or lower (m) 16 bits of a hash of seed and element number say so;
+ * a block whose scale is not above 2^-100 holds zeros.  A root that is held as
+ * zero without being zero is held as 0x80, and the next step divides by the
+ * smallest float (2^-9) times its scale at least.  A state that is not finite is
+ * held as NaN, without a say in its block's scale. */
 int polar_hip_fadamw(polar_hip_device* dev, const polar_hip_adamw_config* config,
                      const polar_hip_adamw_tensor* tensors, uint64_t count);
 

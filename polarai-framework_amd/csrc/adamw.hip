@@ -37,7 +37,7 @@
 
 #include <algorithm>
 #include <cmath>
-#include <new>
+#include <exception>
 #include <utility>
 #include <vector>
 
@@ -344,6 +344,60 @@ template <typename P> Kernel pick(int gradType, bool small) {
                                      : pick<P, TypeBF16>(small);
 }
 
+// What is written must not overlap: a parameter or a state that is listed twice (weights that two
+// layers share) would be updated by two work-groups at once.  Most lists go up in memory field by
+// field, which one pass shows; else the buffers are sorted.
+bool writtenTwice(const polar_hip_adamw_config& config, const polar_hip_adamw_tensor* tensors, uint64_t count) {
+  using Span = std::pair<uintptr_t, uintptr_t>;
+  const bool small = config.state_bits == 8, copy = config.param_type != POLAR_HIP_F32;
+  const uint64_t state = small ? 1 : 4, parameter = sizeOf(config.param_type);
+  auto span = [](const void* at, uint64_t bytes) {
+    return Span{reinterpret_cast<uintptr_t>(at), reinterpret_cast<uintptr_t>(at) + bytes};
+  };
+  constexpr int kFields = 6;
+  auto buffers = [&](const polar_hip_adamw_tensor& t, Span* out) {
+    int n = 0;
+    out[n++] = span(t.param, t.count * parameter);
+    out[n++] = span(t.m, t.count * state);
+    out[n++] = span(t.v, t.count * state);
+    if (copy) out[n++] = span(t.master, t.count * 4);
+    if (small) {
+      const uint64_t blocks = (t.count + kScaleBlock - 1) / kScaleBlock;
+      out[n++] = span(t.m_scale, blocks * 4);
+      out[n++] = span(t.v_scale, blocks * 4);
+    }
+    return n;
+  };
+  auto overlap = [](Span* first, Span* last) {
+    std::sort(first, last);
+    for (Span* s = first; s + 1 < last; ++s)
+      if (s[0].second > s[1].first) return true;
+    return false;
+  };
+  Span area[kFields], mine[kFields]; // of each field
+  bool ascending = true;
+  int fields = 0;
+  for (uint64_t i = 0; i < count && ascending; ++i) {
+    if (tensors[i].count == 0) continue;
+    const bool first = fields == 0;
+    fields = buffers(tensors[i], mine);
+    for (int f = 0; f < fields; ++f) {
+      if (first) area[f] = mine[f];
+      ascending = ascending && (first || mine[f].first >= area[f].second);
+      area[f].second = mine[f].second;
+    }
+  }
+  if (ascending && !overlap(area, area + fields)) return false;
+  std::vector<Span> all;
+  all.reserve(count * kFields);
+  for (uint64_t i = 0; i < count; ++i) {
+    if (tensors[i].count == 0) continue;
+    const int n = buffers(tensors[i], mine);
+    all.insert(all.end(), mine, mine + n);
+  }
+  return overlap(all.data(), all.data() + all.size());
+}
+
 } // namespace
 
 extern "C" {
@@ -375,22 +429,11 @@ int polar_hip_fadamw(polar_hip_device* dev, const polar_hip_adamw_config* config
                           (!small || (alignedTo(t.m_scale, 4) && alignedTo(t.v_scale, 4))),
                       "misaligned pointer");
   }
-  // a parameter that is listed twice (weights that two layers share) would be updated by two work-groups at once
-  if (count > 1) {
-    try {
-      std::vector<std::pair<uintptr_t, uintptr_t>> spans;
-      spans.reserve(count);
-      for (uint64_t i = 0; i < count; ++i) {
-        const uintptr_t at = reinterpret_cast<uintptr_t>(tensors[i].param);
-        if (tensors[i].count != 0) spans.emplace_back(at, at + tensors[i].count * sizeOf(config->param_type));
-      }
-      std::sort(spans.begin(), spans.end());
-      for (size_t i = 1; i < spans.size(); ++i)
-        POLAR_HIP_REQUIRE(spans[i - 1].second <= spans[i].first, "two tensors' parameters overlap");
-    } catch (const std::bad_alloc&) {
-      return fail(POLAR_HIP_ERR_OOM, "polar_hip_fadamw: no host memory to check %llu tensors",
-                  static_cast<unsigned long long>(count));
-    }
+  try {
+    POLAR_HIP_REQUIRE(!writtenTwice(*config, tensors, count), "two of the buffers that are written overlap");
+  } catch (const std::exception&) {
+    return fail(POLAR_HIP_ERR_OOM, "polar_hip_fadamw: no host memory to check %llu tensors",
+                static_cast<unsigned long long>(count));
   }
   POLAR_HIP_TRY(hipSetDevice(dev->ordinal));
   Table table{};
