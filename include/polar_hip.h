@@ -417,7 +417,7 @@ typedef struct polar_hip_adamw_config {
   int state_bits;            /* 32 or 8 */
   uint32_t seed;             /* 8-bit states: of the stochastic rounding; another for each step */
   int64_t step;              /* 1 for the first */
-  double lr, beta1, beta2, eps;
+  double lr, beta1, beta2, eps; /* eps 0, or at least 2^-149; 8-bit states: 2^-126 */
   double grad_scale;         /* gradients are multiplied by it first */
 } polar_hip_adamw_config;
 /* fadamw: one step over `count` tensors, each updated in place:

@@ -415,10 +415,17 @@ int polar_hip_fadamw(polar_hip_device* dev, const polar_hip_adamw_config* config
                         std::isfinite(config->grad_scale),
                     "lr, eps and grad_scale must be finite, eps not negative");
   const bool small = config->state_bits == 8, copy = config->param_type != POLAR_HIP_F32;
+  // the kernel has them in fp32; an eps that is lost there, or (8-bit states) that the hardware's
+  // reciprocal takes for 0, would make 0 / 0 of elements that never had a gradient
+  const double stepSize = config->lr / (1.0 - std::pow(config->beta1, static_cast<double>(config->step)));
+  auto held = [](double x) { return std::isfinite(static_cast<float>(x)); };
+  POLAR_HIP_REQUIRE(held(stepSize) && held(config->grad_scale) && held(config->eps) &&
+                        (config->eps == 0 || config->eps >= (small ? 0x1p-126 : 0x1p-149)),
+                    "lr, grad_scale or eps is out of fp32's range");
   // everything is checked before the first tensor is touched
   for (uint64_t i = 0; i < count; ++i) {
     const polar_hip_adamw_tensor& t = tensors[i];
-    POLAR_HIP_REQUIRE(std::isfinite(t.weight_decay), "a tensor's weight decay is not finite");
+    POLAR_HIP_REQUIRE(held(config->lr * t.weight_decay), "lr times a tensor's weight decay is out of fp32's range");
     if (t.count == 0) continue;
     POLAR_HIP_REQUIRE(t.count <= kChunk * kMostGroups, "a tensor is too large");
     POLAR_HIP_REQUIRE(t.param && t.grad && t.m && t.v, "a tensor's pointer is null");
@@ -437,14 +444,13 @@ int polar_hip_fadamw(polar_hip_device* dev, const polar_hip_adamw_config* config
   }
   POLAR_HIP_TRY(hipSetDevice(dev->ordinal));
   Table table{};
-  const double correction1 = 1.0 - std::pow(config->beta1, static_cast<double>(config->step));
   const double correction2 = 1.0 - std::pow(config->beta2, static_cast<double>(config->step));
   table.gradScale = static_cast<float>(config->grad_scale);
   table.beta1 = static_cast<float>(config->beta1);
   table.rest1 = static_cast<float>(1.0 - config->beta1);
   table.beta2 = static_cast<float>(config->beta2);
   table.rest2 = static_cast<float>(1.0 - config->beta2);
-  table.stepSize = static_cast<float>(config->lr / correction1);
+  table.stepSize = static_cast<float>(stepSize);
   table.byCorrection = static_cast<float>(1.0 / std::sqrt(correction2));
   table.eps = static_cast<float>(config->eps);
   table.seed = config->seed;

@@ -49,3 +49,12 @@ def test_adamw_refuses_a_master_that_is_the_copy(lib, handle):  # noqa: F811
     only = tensor(0)
     only["master"] = only["param"]
     refused(lib, step(lib, handle, [only], param_type=1), "overlap")
+
+
+@pytest.mark.parametrize("change", [dict(lr=1e300), dict(lr=1e38, beta1=0.999), dict(grad_scale=-1e39), dict(eps=1e39), dict(eps=1e-46), dict(eps=1e-39, state_bits=8)])
+def test_adamw_refuses_settings_that_fp32_does_not_hold(lib, handle, change):  # noqa: F811
+    refused(lib, step(lib, handle, [tensor(0)], **change), "fp32")
+
+
+def test_adamw_refuses_a_decay_that_fp32_does_not_hold(lib, handle):  # noqa: F811
+    refused(lib, step(lib, handle, [tensor(0), tensor(1, weight_decay=1e60)]), "decay")
