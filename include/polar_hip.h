@@ -329,7 +329,8 @@ int polar_hip_fsigmoid_flogloss(polar_hip_device* dev, const float* in,
  * element, the distance of two rows' first elements (its stride, in elements,
  * at least cols) and rows x cols, and its elements behind cols in a row are
  * neither read nor written.  Pointers need the alignment of one element.  Rows
- * may be none; then nothing is done. */
+ * may be none; then nothing is done, but for flayernorm_grad's dweight and dbias:
+ * sums over no rows, zeros. */
 typedef enum polar_hip_type { POLAR_HIP_F32 = 0, POLAR_HIP_F16 = 1, POLAR_HIP_BF16 = 2 } polar_hip_type;
 /* Tokens: whole numbers, also as fp32 (the framework's tensors hold nothing else) */
 typedef enum polar_hip_index_type {

@@ -657,7 +657,7 @@ int polar_hip_flayernorm_grad(polar_hip_device* dev, int type, const void* dy, u
   POLAR_HIP_REQUIRE(cols >= 1 && cols <= kMaxCols, "rows of 1 to 2^24 elements");
   POLAR_HIP_REQUIRE(rows < (1ull << 31), "too many rows");
   POLAR_HIP_REQUIRE(rows == 0 || (dy && x), "null tensor");
-  POLAR_HIP_REQUIRE(dyStride >= cols && xStride >= cols && (dx == nullptr || dxStride >= cols),
+  POLAR_HIP_REQUIRE(rows == 0 || (dyStride >= cols && xStride >= cols && (dx == nullptr || dxStride >= cols)),
                     "a row's stride is shorter than the row");
   POLAR_HIP_REQUIRE(addressable(rows, std::max({dyStride, xStride, dx ? dxStride : 0}), sizeOf(type)), "tensor too large");
   POLAR_HIP_REQUIRE(alignedTo(dy, sizeOf(type)) && alignedTo(x, sizeOf(type)) && alignedTo(dx, sizeOf(type)) &&

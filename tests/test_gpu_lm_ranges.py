@@ -116,6 +116,15 @@ def test_layernorm_grad_of_constant_rows_far_from_zero(dev, kind, cols, given):
         t.free()
 
 
+@pytest.mark.parametrize("params", ["f32", "bf16"])
+def test_layernorm_grad_over_no_rows_asks_for_no_strides(dev, params):
+    _say("flayernorm_grad no rows, no strides")
+    DW, DB = (Raw(dev, np.ones(70, ref.STORED[params])) for _ in range(2))
+    dev.flayernorm_grad(None, None, None, None, DW, DB, 0, 70, dtype=params, param_dtype=params, grad_stride=0, x_stride=0)
+    assert not DW.values().any() and not DB.values().any()
+    DW.free(), DB.free()
+
+
 # ---- AdamW ------------------------------------------------------------------------
 
 def test_adamw_8_bit_states_with_seven_decades_in_a_block(dev):

@@ -5,7 +5,7 @@ import ctypes as C
 import pytest
 
 from polarai_framework_amd import capi
-from test_lm_operators import A, CONFIG, TENSOR, handle, lib, refused  # noqa: F401  (fixtures)
+from test_lm_operators import A, CONFIG, NORM_GRAD, TENSOR, handle, lib, refused  # noqa: F401  (fixtures)
 
 
 def tensor(i, **change):
@@ -58,3 +58,8 @@ def test_adamw_refuses_settings_that_fp32_does_not_hold(lib, handle, change):  #
 
 def test_adamw_refuses_a_decay_that_fp32_does_not_hold(lib, handle):  # noqa: F811
     refused(lib, step(lib, handle, [tensor(0), tensor(1, weight_decay=1e60)]), "decay")
+
+
+def test_layernorm_grad_over_no_rows_takes_any_strides(lib, handle):  # noqa: F811
+    call = {**NORM_GRAD, "dev": handle, "rows": 0, "dx": 0, "dweight": 0, "dbias": 0, "dyStride": 0, "xStride": 3, "dxStride": 0}
+    assert lib.polar_hip_flayernorm_grad(*call.values()) == 0
