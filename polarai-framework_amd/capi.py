@@ -79,6 +79,8 @@ class AdamWConfig(C.Structure):
 TYPES = {"f32": 0, "f16": 1, "bf16": 2}         # polar_hip_type
 INDEX_TYPES = {"i32": 0, "i64": 1, "f32": 2}    # polar_hip_index_type
 STATE_BITS = {"f32": 32, "8bit": 8}
+SIZES = {"f32": 4, "f16": 2, "bf16": 2}         # bytes of an element
+INDEX_SIZES = {"i32": 4, "i64": 8, "f32": 4}
 LOGPROB_MAX_TOP = 32
 ADAMW_BLOCK = 256
 
@@ -176,28 +178,69 @@ def _check(lib, status):
         raise PolarHipError(status, lib.polar_hip_last_error().decode())
 
 
-def _ptr(x):
+def _ptr(x, name, nbytes, ordinal):
     """Device address of a Buffer, of a tensor of another library on the same GPU (anything with data_ptr()), or of
     a plain address; None stays None.  The device's stream is its own: work of another library on such a tensor is
-    waited for before the call, and the call before that library uses the tensor again."""
-    if x is None or isinstance(x, int):
+    waited for before the call, and the call before that library uses the tensor again.  A tensor that says where it
+    lies (get_device()) and what it holds (nbytes) is refused on another device, or with less than `nbytes` bytes: a
+    kernel would access memory that is not its own."""
+    if x is None:
+        return None
+    kind = x.__class__
+    if kind is int:
         return x
-    at = getattr(x, "ptr", None)
-    return x.data_ptr() if at is None else at
+    if kind is Buffer:
+        return x.ptr
+    try:
+        if x.get_device() == ordinal and x.nbytes >= nbytes:
+            return x.data_ptr()
+    except AttributeError:
+        if isinstance(x, int):
+            return x
+        at = getattr(x, "ptr", None)
+        return x.data_ptr() if at is None else at
+    _check_place(x, name, x.get_device(), ordinal)
+    if x.nbytes < nbytes:
+        raise ValueError(f"{name} holds {x.nbytes} bytes, {nbytes} are needed (its dtype, rows or columns?)")
+    return x.data_ptr()
+
+
+def _check_place(x, name, where, ordinal):
+    """Refuses a tensor that does not lie on device `ordinal`; pinned host memory is accessible from all of them."""
+    if where < 0:
+        pinned = getattr(x, "is_pinned", None)
+        if pinned is None or not pinned():
+            raise TypeError(f"{name} is not in device memory")
+    elif where != ordinal:
+        raise TypeError(f"{name} lies on device {where}, the call is made on device {ordinal}")
 
 
 def adamw_tensors(tensors):
     """The list of tensors that Device.fadamw takes, from dicts with the fields of polar_hip_adamw_tensor (those left
     out or None are null; weight_decay is 0).  A training program makes it once."""
     table = (AdamWTensor * len(tensors))()
+    # for fadamw, which knows device and types: a field for each device that a tensor lies on, and for each field the
+    # fewest bytes that one of its tensors holds per element (of the scales, per block)
+    table.places, table.room = {}, {}
     for entry, t in zip(table, tensors):
+        count = int(t.get("count", 0))
         for name, value in t.items():
             if name in ("count", "first"):
                 setattr(entry, name, int(value))
             elif name == "weight_decay":
                 entry.weight_decay = value
             elif name in ("param", "grad", "m", "v", "master", "m_scale", "v_scale"):
-                setattr(entry, name, _ptr(value))
+                where = value.get_device() if hasattr(value, "get_device") and hasattr(value, "nbytes") else None
+                setattr(entry, name, _ptr(value, name, 0, where))
+                if where is None:
+                    continue
+                if where < 0:
+                    _check_place(value, name, where, where)
+                else:
+                    table.places[where] = name
+                units = -(-count // ADAMW_BLOCK) if name.endswith("scale") else count
+                if units:
+                    table.room[name] = min(table.room.get(name, 1 << 62), value.nbytes // units)
             else:
                 raise KeyError(f"no field {name} in a tensor of fadamw")
     return table
@@ -280,6 +323,7 @@ class Device:
         h = _vp()
         _check(self.lib, self.lib.polar_hip_device_open(ordinal, C.byref(h)))
         self.handle = h
+        self.ordinal = ordinal
 
     # -- lifetime -----------------------------------------------------------
     def close(self):
@@ -445,35 +489,55 @@ class Device:
     # tensors are Buffers, tensors of another library, or device addresses (_ptr)
     def flayernorm(self, x, weight, bias, out, rows, cols, eps=1e-5, mean=None, rstd=None, dtype="f32",
                    param_dtype="f32", x_stride=None, out_stride=None):
+        at, whole, params, stats = self.ordinal, rows * cols * SIZES[dtype], cols * SIZES[param_dtype], rows * 4
         _check(self.lib, self.lib.polar_hip_flayernorm(
-            self.handle, TYPES[dtype], _ptr(x), cols if x_stride is None else x_stride, TYPES[param_dtype],
-            _ptr(weight), _ptr(bias), eps, _ptr(out), cols if out_stride is None else out_stride, _ptr(mean),
-            _ptr(rstd), rows, cols))
+            self.handle, TYPES[dtype], _ptr(x, "x", whole, at), cols if x_stride is None else x_stride,
+            TYPES[param_dtype], _ptr(weight, "weight", params, at), _ptr(bias, "bias", params, at), eps,
+            _ptr(out, "out", whole, at), cols if out_stride is None else out_stride, _ptr(mean, "mean", stats, at),
+            _ptr(rstd, "rstd", stats, at), rows, cols))
 
     def flayernorm_grad(self, grad, x, weight, dx, dweight, dbias, rows, cols, eps=1e-5, mean=None, rstd=None,
                         dtype="f32", param_dtype="f32", grad_stride=None, x_stride=None, dx_stride=None):
+        at, whole, params, stats = self.ordinal, rows * cols * SIZES[dtype], cols * SIZES[param_dtype], rows * 4
         _check(self.lib, self.lib.polar_hip_flayernorm_grad(
-            self.handle, TYPES[dtype], _ptr(grad), cols if grad_stride is None else grad_stride, _ptr(x),
-            cols if x_stride is None else x_stride, TYPES[param_dtype], _ptr(weight), _ptr(mean), _ptr(rstd), eps,
-            _ptr(dx), cols if dx_stride is None else dx_stride, _ptr(dweight), _ptr(dbias), rows, cols))
+            self.handle, TYPES[dtype], _ptr(grad, "grad", whole, at), cols if grad_stride is None else grad_stride,
+            _ptr(x, "x", whole, at), cols if x_stride is None else x_stride, TYPES[param_dtype],
+            _ptr(weight, "weight", params, at), _ptr(mean, "mean", stats, at), _ptr(rstd, "rstd", stats, at), eps,
+            _ptr(dx, "dx", whole, at), cols if dx_stride is None else dx_stride, _ptr(dweight, "dweight", params, at),
+            _ptr(dbias, "dbias", params, at), rows, cols))
 
     def flogprob(self, logits, tokens, logprob, rows, cols, scale=1.0, stats=None, entropy=None, top=0, top_index=None,
                  top_logprob=None, dtype="f32", token_dtype="i64", stride=None):
+        at, each, best = self.ordinal, rows * 4, rows * top * 4
         _check(self.lib, self.lib.polar_hip_flogprob(
-            self.handle, TYPES[dtype], _ptr(logits), cols if stride is None else stride, INDEX_TYPES[token_dtype],
-            _ptr(tokens), scale, _ptr(logprob), _ptr(stats), _ptr(entropy), top, _ptr(top_index), _ptr(top_logprob),
-            rows, cols))
+            self.handle, TYPES[dtype], _ptr(logits, "logits", rows * cols * SIZES[dtype], at),
+            cols if stride is None else stride, INDEX_TYPES[token_dtype],
+            _ptr(tokens, "tokens", rows * INDEX_SIZES[token_dtype], at), scale, _ptr(logprob, "logprob", each, at),
+            _ptr(stats, "stats", 2 * each, at), _ptr(entropy, "entropy", each, at), top,
+            _ptr(top_index, "top_index", best, at), _ptr(top_logprob, "top_logprob", best, at), rows, cols))
 
     def flogprob_grad(self, logits, tokens, stats, dlogprob, dlogits, rows, cols, scale=1.0, entropy=None,
                       dentropy=None, dtype="f32", token_dtype="i64", stride=None, dlogits_stride=None):
+        at, each, whole = self.ordinal, rows * 4, rows * cols * SIZES[dtype]
         _check(self.lib, self.lib.polar_hip_flogprob_grad(
-            self.handle, TYPES[dtype], _ptr(logits), cols if stride is None else stride, INDEX_TYPES[token_dtype],
-            _ptr(tokens), scale, _ptr(stats), _ptr(dlogprob), _ptr(entropy), _ptr(dentropy), _ptr(dlogits),
-            cols if dlogits_stride is None else dlogits_stride, rows, cols))
+            self.handle, TYPES[dtype], _ptr(logits, "logits", whole, at), cols if stride is None else stride,
+            INDEX_TYPES[token_dtype], _ptr(tokens, "tokens", rows * INDEX_SIZES[token_dtype], at), scale,
+            _ptr(stats, "stats", 2 * each, at), _ptr(dlogprob, "dlogprob", each, at),
+            _ptr(entropy, "entropy", each, at), _ptr(dentropy, "dentropy", each, at),
+            _ptr(dlogits, "dlogits", whole, at), cols if dlogits_stride is None else dlogits_stride, rows, cols))
 
     def fadamw(self, tensors, step, lr, beta1=0.9, beta2=0.999, eps=1e-8, grad_scale=1.0, seed=0, dtype="f32",
                grad_dtype="f32", state_dtype="f32"):
         """`tensors`: what adamw_tensors() made."""
+        for where, name in getattr(tensors, "places", {}).items():
+            _check_place(None, name, where, self.ordinal)
+        state, scale = (1, 4) if state_dtype == "8bit" else (4, 0)
+        need = dict(param=SIZES[dtype], grad=SIZES[grad_dtype], m=state, v=state, master=0 if dtype == "f32" else 4,
+                    m_scale=scale, v_scale=scale)
+        for name, room in getattr(tensors, "room", {}).items():
+            if room < need[name]:
+                raise ValueError(f"a tensor's {name} is too short: {room} bytes for each of its elements or blocks, "
+                                 f"{need[name]} are needed")
         config = AdamWConfig(TYPES[dtype], TYPES[grad_dtype], STATE_BITS[state_dtype], seed, step, lr, beta1, beta2, eps,
                              grad_scale)
         _check(self.lib, self.lib.polar_hip_fadamw(self.handle, C.byref(config), tensors, len(tensors)))

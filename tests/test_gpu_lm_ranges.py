@@ -7,7 +7,7 @@ import pytest
 import lm_reference as ref
 from lm_reference import U32, Matrix, Raw
 from polarai_framework_amd import capi
-from test_gpu_lm_operators import close, logprob_tolerances
+from test_gpu_lm_operators import close, logprob_tolerances, norm_tolerances
 
 pytestmark = pytest.mark.gpu
 
@@ -192,3 +192,37 @@ def test_adamw_8_bit_roots_below_the_smallest_code(dev):
     assert np.abs(step[1:100] - want).max() <= 20 * U32 * want + 4 * U32 * np.abs(before[1:100]).max()
     for t in (P, G, M, V, MS, VS):
         t.free()
+
+
+# ---- tensors of another library ---------------------------------------------------
+
+def test_tensors_of_another_library(dev):
+    """Device and pinned host memory of torch; what is too short for its type or lies in ordinary host memory is refused before
+    a kernel sees it."""
+    torch = pytest.importorskip("torch")
+    _say("torch tensors")
+    rng = np.random.default_rng(2)
+    rows, cols = 5, 300
+    x = ref.rounded(rng.standard_normal((rows, cols)), "bf16")
+    X = torch.tensor(x, dtype=torch.bfloat16, device="cuda")
+    Y = torch.empty(rows, cols, dtype=torch.bfloat16, device="cuda")
+    W = torch.ones(cols).pin_memory()
+    torch.cuda.synchronize()
+    dev.flayernorm(X, W, None, Y, rows, cols, dtype="bf16")
+    dev.synchronize()
+    y, mean, rstd = ref.layernorm(x, np.ones(cols), 0.0, 1e-5)
+    close(Y.double().cpu().numpy(), y, norm_tolerances(x, np.ones(cols), np.zeros(cols), y, mean, rstd, "bf16")[0], "y")
+    with pytest.raises(ValueError, match="x holds 3000 bytes, 6000"):
+        dev.flayernorm(X, None, None, torch.empty(rows, cols, device="cuda"), rows, cols)
+    with pytest.raises(TypeError, match="weight"):
+        dev.flayernorm(X, torch.ones(cols), None, Y, rows, cols, dtype="bf16")
+    with pytest.raises(ValueError, match="tokens"):
+        dev.flogprob(X, torch.zeros(rows, dtype=torch.int32, device="cuda"), Y, rows, cols, dtype="bf16")
+    p, g, m, v = (torch.full((100,), c, device="cuda") for c in (1.0, 0.5, 0.0, 0.0))
+    torch.cuda.synchronize()
+    plan = capi.adamw_tensors([dict(count=100, param=p, grad=g, m=m, v=v)])
+    with pytest.raises(ValueError, match="grad"):
+        dev.fadamw(capi.adamw_tensors([dict(count=100, param=p, grad=g.bfloat16(), m=m, v=v)]), step=1, lr=1e-3)
+    dev.fadamw(plan, step=1, lr=1e-3)
+    dev.synchronize()
+    assert np.abs(p.cpu().numpy() - (1 - 1e-3)).max() <= 4 * U32
