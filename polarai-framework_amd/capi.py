@@ -217,11 +217,12 @@ def _check_place(x, name, where, ordinal):
 
 def adamw_tensors(tensors):
     """The list of tensors that Device.fadamw takes, from dicts with the fields of polar_hip_adamw_tensor (those left
-    out or None are null; weight_decay is 0).  A training program makes it once."""
+    out or None are null; weight_decay is 0).  A training program makes it once; it keeps what it was given alive.
+    Where a gradient moves from step to step, its address is put into the list: plan[i].grad = gradient.data_ptr()."""
     table = (AdamWTensor * len(tensors))()
     # for fadamw, which knows device and types: a field for each device that a tensor lies on, and for each field the
     # fewest bytes that one of its tensors holds per element (of the scales, per block)
-    table.places, table.room = {}, {}
+    table.kept, table.places, table.room = [], {}, {}
     for entry, t in zip(table, tensors):
         count = int(t.get("count", 0))
         for name, value in t.items():
@@ -232,6 +233,9 @@ def adamw_tensors(tensors):
             elif name in ("param", "grad", "m", "v", "master", "m_scale", "v_scale"):
                 where = value.get_device() if hasattr(value, "get_device") and hasattr(value, "nbytes") else None
                 setattr(entry, name, _ptr(value, name, 0, where))
+                if value is None or isinstance(value, int):
+                    continue
+                table.kept.append(value)
                 if where is None:
                     continue
                 if where < 0:

@@ -1,6 +1,8 @@
 """CPU tests of how the language-model operators are called: what is refused because two tensors of AdamW would be written by
 two work-groups at once, settings that fp32 does not hold, calls over no rows, and operands of other libraries."""
 import ctypes as C
+import gc
+import weakref
 
 import pytest
 
@@ -138,6 +140,19 @@ def test_strided_rows_need_no_more_than_their_elements():
     assert len(dev.calls) == 2
 
 
+def test_adamw_lists_keep_their_tensors():
+    """The list is made once and used at every step: what it points to lives as long as it does."""
+    made = Foreign(nbytes=12)
+    alive = weakref.ref(made)
+    plan = capi.adamw_tensors([dict(count=3, param=made, grad=A, m=A, v=A)])
+    del made
+    gc.collect()
+    assert alive() is not None and plan[0].param == A
+    del plan
+    gc.collect()
+    assert alive() is None
+
+
 def test_adamw_lists_are_checked_against_the_device_and_the_call():
     dev = Recorder()
     config = dict(step=1, lr=1e-3)
@@ -159,3 +174,12 @@ def test_adamw_lists_are_checked_against_the_device_and_the_call():
         dev.fadamw(capi.adamw_tensors([dict(count=300, param=A, grad=A, m=A, v=A, m_scale=Foreign(nbytes=4), v_scale=A)]),
                    state_dtype="8bit", **config)
     assert len(dev.calls) == 3
+
+
+def test_adamw_lists_take_new_gradients():
+    """A gradient that moved: its address is put into the list."""
+    plan = capi.adamw_tensors([dict(count=3, param=A, grad=A, m=A, v=A)])
+    plan[0].grad = A + 64
+    dev = Recorder()
+    dev.fadamw(plan, step=1, lr=1e-3)
+    assert dev.calls[0][1][2][0].grad == A + 64
