@@ -116,6 +116,85 @@ def test_layernorm_grad_of_constant_rows_far_from_zero(dev, kind, cols, given):
         t.free()
 
 
+@pytest.mark.parametrize("rows,cols,kind", [(13000, 40, "f32"), (13000, 513, "bf16"), (12600, 300, "f32"), (6200, 1500, "f16"), (6200, 700, "f32"),
+                                            (2100, 4000, "bf16"), (2100, 2000, "f32"), (1300, 8192, "bf16"), (1300, 4000, "f32"),
+                                            (600, 16384, "bf16"), (600, 8000, "f32"), (600, 16384, "f32")])
+def test_layernorm_of_several_rows_per_team(dev, rows, cols, kind):
+    """More rows than the grid has teams and each of them rows ahead: the registers of the rows that come next are filled
+    again and the walk ends inside a round."""
+    _say("flayernorm rows per team", rows, cols, kind)
+    rng = np.random.default_rng(rows + cols)
+    x = ref.rounded(rng.standard_normal((rows, cols)) * 1.5 + rng.standard_normal((rows, 1)) * 3, kind)
+    w, b = ref.rounded(1 + 0.3 * rng.standard_normal(cols), "f32"), ref.rounded(0.5 * rng.standard_normal(cols), "f32")
+    y, mean, rstd = ref.layernorm(x, w, b, 1e-5)
+    X, Y = Matrix(dev, kind, rows, cols, cols + 3, 1, x), Matrix(dev, kind, rows, cols, cols + 1, 2)
+    W, B = Raw(dev, w.astype(np.float32)), Raw(dev, b.astype(np.float32))
+    M, R = Raw(dev, np.zeros(rows, np.float32)), Raw(dev, np.zeros(rows, np.float32))
+    dev.flayernorm(X, W, B, Y, rows, cols, mean=M, rstd=R, dtype=kind, x_stride=X.stride, out_stride=Y.stride)
+    y_tol, mean_tol, rstd_tol = norm_tolerances(x, w, b, y, mean, rstd, kind)
+    close(Y.values(), y, y_tol, "y")
+    close(M.values(), mean, mean_tol, "mean")
+    close(R.values(), rstd, rstd_tol, "rstd")
+    for t in (X, Y, W, B, M, R):
+        t.free()
+
+
+def norm_error_bounds(x, w, mean, rstd, given):
+    """(mean_tol, rstd_rel) as in test_gpu_lm_operators: none where the statistics are given."""
+    if given:
+        return np.zeros((len(x), 1)), np.zeros((len(x), 1))
+    mean_tol = 64 * U32 * np.abs(x).mean(1)
+    return mean_tol[:, None], (64 * U32 + 0.5 * (rstd * mean_tol) ** 2)[:, None]
+
+
+def check_norm_grad(dev, x, dy, w, kind, params, given, eps=1e-3):
+    rows, cols = x.shape
+    _, mean, rstd = ref.layernorm(x, w, 0.0, eps)
+    mean32, rstd32 = mean.astype(np.float32), rstd.astype(np.float32)
+    mean_, rstd_ = (mean32.astype(np.float64), rstd32.astype(np.float64)) if given else (mean, rstd)
+    dx, dw, db = ref.layernorm_grad(dy, x, w, mean_, rstd_)
+    mean_tol, rstd_rel = norm_error_bounds(x, w, mean, rstd, given)
+    h = np.abs(x - mean_[:, None]) * rstd_[:, None]
+    h_tol = rstd_[:, None] * mean_tol + h * (rstd_rel + 3 * U32) + rstd_[:, None] * 2 * U32 * np.abs(mean_[:, None])
+    g = np.abs(dy * w)
+    along1, alongh = g.mean(1, keepdims=True), (g * h).mean(1, keepdims=True)
+    alongh_tol = (g * h_tol).mean(1, keepdims=True) + 64 * U32 * alongh
+    dx_tol = rstd_[:, None] * (4 * U32 * (g + along1 + h * alongh) + 64 * U32 * along1 + h * alongh_tol + h_tol * alongh)
+    dx_tol = dx_tol + np.abs(dx) * (rstd_rel + 2 * U32)
+    adds = 32 + rows
+    dw_tol = adds * U32 * (np.abs(dy) * h).sum(0) + (np.abs(dy) * h_tol).sum(0)
+    db_tol = adds * U32 * np.abs(dy).sum(0)
+    DY, X = Matrix(dev, kind, rows, cols, cols + 2, 3, dy), Matrix(dev, kind, rows, cols, cols + 5, 2, x)
+    W, M, R = Raw(dev, ref.store(w, params)), Raw(dev, mean32), Raw(dev, rstd32)
+    DX = Matrix(dev, kind, rows, cols, cols + 1, 7)
+    DW, DB = (Raw(dev, np.zeros(cols, ref.STORED[params])) for _ in range(2))
+    dev.flayernorm_grad(DY, X, W, DX, DW, DB, rows, cols, eps=eps, mean=M if given else None, rstd=R if given else None, dtype=kind,
+                        param_dtype=params, grad_stride=DY.stride, x_stride=X.stride, dx_stride=DX.stride)
+    half = ref.HALF_STEP
+
+    def stored(want, k):
+        return half[k] * np.abs(want) + ref.TINY[k]
+    close(DX.values(), dx, dx_tol * (1 + half[kind]) + stored(dx, kind), "dx")
+    close(ref.widen(DW.values(), params), dw, dw_tol * 1.01 + stored(dw, params), "dweight")
+    close(ref.widen(DB.values(), params), db, db_tol * 1.01 + stored(db, params), "dbias")
+    for t in (DY, X, W, M, R, DX, DW, DB):
+        t.free()
+
+
+@pytest.mark.parametrize("rows,cols,kind", [(8300, 40, "f32"), (8300, 600, "bf16"), (8300, 300, "f32"), (1600, 2000, "f16"), (1600, 1000, "f32"),
+                                            (1300, 4096, "bf16"), (1300, 2048, "f32"), (800, 8192, "bf16"), (800, 4000, "f32"),
+                                            (600, 16384, "bf16"), (600, 8192, "f32"), (600, 16384, "f32"), (100, 33000, "bf16"), (100, 33000, "f32")])
+@pytest.mark.parametrize("given", [True, False])
+def test_layernorm_grad_of_several_rows_per_team(dev, rows, cols, kind, given):
+    """As above; every team adds several rows to its columns' sums, in registers and in LDS, and a slice of long rows has
+    several of them."""
+    _say("flayernorm_grad rows per team", rows, cols, kind, given)
+    rng = np.random.default_rng(rows + cols + 1)
+    x = ref.rounded(rng.standard_normal((rows, cols)) * 1.5 + rng.standard_normal((rows, 1)) * 3, kind)
+    w = ref.rounded(1 + 0.3 * rng.standard_normal(cols), "f32")
+    check_norm_grad(dev, x, ref.rounded(rng.standard_normal((rows, cols)), kind), w, kind, "f32", given)
+
+
 @pytest.mark.parametrize("params", ["f32", "bf16"])
 def test_layernorm_grad_over_no_rows_asks_for_no_strides(dev, params):
     _say("flayernorm_grad no rows, no strides")
@@ -192,6 +271,40 @@ def test_adamw_8_bit_roots_below_the_smallest_code(dev):
     assert np.abs(step[1:100] - want).max() <= 20 * U32 * want + 4 * U32 * np.abs(before[1:100]).max()
     for t in (P, G, M, V, MS, VS):
         t.free()
+
+
+def test_adamw_8_bit_lists_over_launches_and_far_element_numbers(dev):
+    """More tensors than a launch takes, whose elements' numbers in the random sequence lie beyond 2^32, and for one of them on
+    both sides of it: each state within the neighbours that its own random bits allow."""
+    _say("fadamw numbers")
+    rng = np.random.default_rng(55)
+    sizes = [1, 255, 256, 257, 1023, 4097, 7] * 15
+    firsts = [[0, (1 << 32) - 100, (1 << 32) + 5, (1 << 40) + 123, (1 << 63) + 1][i % 5] for i in range(len(sizes))]
+    made, fields = [], []
+    for n, first in zip(sizes, firsts):
+        g, p = (rng.standard_normal(n) * 0.1).astype(np.float32), rng.standard_normal(n).astype(np.float32)
+        blocks = -(-n // 256)
+        t = dict(n=n, first=first, g=g, G=Raw(dev, g), P=Raw(dev, p), M=Raw(dev, np.zeros(n, np.uint8)), V=Raw(dev, np.zeros(n, np.uint8)),
+                 MS=Raw(dev, np.zeros(blocks, np.float32)), VS=Raw(dev, np.zeros(blocks, np.float32)))
+        made.append(t)
+        fields.append(dict(count=n, first=first, param=t["P"], grad=t["G"], m=t["M"], v=t["V"], m_scale=t["MS"], v_scale=t["VS"]))
+    dev.fadamw(capi.adamw_tensors(fields), step=1, lr=1e-3, seed=99, state_dtype="8bit")
+    for t in made:
+        n, wide = t["n"], t["g"].astype(np.float64)
+        number = (np.uint64(t["first"]) + np.arange(n, dtype=np.uint64))
+        bits = ref.random_bits(99, number)
+        for codes, scales, new, random in ((t["M"], t["MS"], 0.1 * wide, bits & np.uint64(0xFFFF)),
+                                           (t["V"], t["VS"], np.sqrt(0.001) * np.abs(wide), bits >> np.uint64(16))):
+            by = np.arange(n) // 256
+            scale = scales.values().astype(np.float64)
+            close(scale, ref.block_largest(new) / 448, 8 * U32 * ref.block_largest(new) / 448, "scale")
+            at, unit = ref.held_in_8_bits(new, scale[by], random.astype(np.float64))
+            near = 10 * U32 * np.abs(new) / scale[by] / unit + 2.0 ** -20
+            low, high = np.floor(at - near) * unit, np.floor(at + near) * unit
+            got = np.abs(ref.E4M3[codes.values()])
+            assert ((got >= np.minimum(low, 448)) & (got <= np.minimum(high, 448))).all(), (n, t["first"])
+        for k in ("G", "P", "M", "V", "MS", "VS"):
+            t[k].free()
 
 
 # ---- tensors of another library ---------------------------------------------------
