@@ -172,9 +172,12 @@ __device__ __forceinline__ uint32_t randomBits(uint32_t seed, uint64_t element) 
 }
 
 // The square root, rounded to nearest: the hardware's is good to a unit in the last
-// place, and the sign of what its two neighbours leave over says which of the three it
-// is.  Exact where that rest is a normal number (v from 2^-96 on), else as the hardware
-// has it; 0, infinity and NaN stay what they are.
+// place, and Tuckerman's test (published with IBM's elementary functions for the
+// System/370, 1986) says which of it and its two neighbours it is: the sign of what
+// neighbour * r leaves of v, by a fused multiply-add.  The compiler refines sqrtf by the
+// same test, with a scaling of small arguments that is left out here: exact where that
+// rest is a normal number (v from 2^-96 on), else as the hardware has it; 0, infinity and
+// NaN stay what they are.
 __device__ __forceinline__ float rootOf(float v) {
   const float r = __builtin_amdgcn_sqrtf(v);
   const float below = __builtin_bit_cast(float, __builtin_bit_cast(uint32_t, r) - 1u);

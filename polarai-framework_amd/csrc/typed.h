@@ -121,16 +121,11 @@ __device__ __forceinline__ void storePack(typename T::Stored* row, uint64_t c, u
 // vector is absent (null) and behind its end.
 template <typename P, int kCount>
 __device__ __forceinline__ void loadParams(const typename P::Stored* v, uint64_t c, uint64_t cols, float fill, float* out) {
-  static_assert(kCount % P::kVec == 0 || kCount == 4, "whole packs, or half a pack of 16-bit parameters");
+  static_assert(kCount % P::kVec == 0, "whole packs");
   if (v != nullptr && c + kCount <= cols) {
-    if constexpr (kCount % P::kVec == 0) {
 #pragma unroll
-      for (int k = 0; k < kCount / P::kVec; ++k)
-        P::unpack(*reinterpret_cast<const typename P::At*>(v + c + k * P::kVec), out + k * P::kVec);
-    } else {
-#pragma unroll
-      for (int i = 0; i < kCount; ++i) out[i] = P::widen(v[c + i]);
-    }
+    for (int k = 0; k < kCount / P::kVec; ++k)
+      P::unpack(*reinterpret_cast<const typename P::At*>(v + c + k * P::kVec), out + k * P::kVec);
   } else {
 #pragma unroll
     for (int i = 0; i < kCount; ++i) out[i] = v != nullptr && c + i < cols ? P::widen(v[c + i]) : fill;
