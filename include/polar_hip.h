@@ -425,7 +425,7 @@ typedef struct polar_hip_adamw_config {
  *   g = grad_scale * grad;  m = beta1 m + (1 - beta1) g;  v = beta2 v + (1 - beta2) g^2
  *   param = param - lr weight_decay param
  *           - lr / (1 - beta1^step) m / (sqrt(v) / sqrt(1 - beta2^step) + eps)
- * The list is read before the call returns.  All of it is checked before
+ * (with eps 0 an element that never had a gradient becomes 0 / 0, NaN).  The list is read before the call returns.  All of it is checked before
  * anything is launched.  Buffers that are written must not overlap and are
  * refused if they do (weights that two layers share are listed once), nor may a
  * gradient overlap one of them.  8-bit states are rounded stochastically, up where

@@ -4,9 +4,9 @@
 //   p = p - lr wd p - (lr / (1 - b1^t)) m / (sqrt(v) / sqrt(1 - b2^t) + eps)
 //
 // Everything is read once and written once: memory is what bounds it.  100
-// million elements in fp32 (28 bytes each) take 457 us, 6.2 TB/s, 90 % of what
+// million elements in fp32 (28 bytes each) take 456 us, 6.2 TB/s, 90 % of what
 // a large copy reaches; 260 million with states in 8 bits, bf16 gradients and
-// copies (16 bytes each) 705 us, 6.1 TB/s.  Loads and stores stream past the
+// copies (16 bytes each) 693 us, 6.2 TB/s.  Loads and stores stream past the
 // caches (with plain loads or plain stores 510 us).  A launch covers up to
 // kTensors tensors, whose table travels in the kernel's arguments: no table in
 // device memory to upload and keep, and a model of a few hundred tensors takes
@@ -30,9 +30,9 @@
 // rounds to zero therefore leaves a trace, code 0x80 (minus zero: it still counts
 // as 0 for the next root, so that the average is kept), and the next step divides
 // by the smallest code at least: too small a step, as with a larger eps, in place
-// of one that is too large (elements 10^6 times below the largest of their block
-// over 1500 steps: root mean square 0.15 lr and at most 1.5 lr, with states in 32
-// bits 0.23 and 1.1, without the trace 8.3 and 399).
+// of one that is too large (emulated, 1500 steps of elements 10^6 times below the
+// largest of their block: root mean square 0.15 lr and at most 1.5 lr, with states
+// in 32 bits 0.23 and 1.1, without the trace 8.3 and 399).
 #include "typed.h"
 
 #include <algorithm>
